@@ -28,6 +28,8 @@ import torch.nn.functional as F
 
 import logging
 
+from .utils import captured
+
 
 logger = logging.getLogger(__name__)
 # the encoder's linear layers through the split GEMM as well (False: HF's own encoder layers, fp32 library GEMMs; the tests flip it)
@@ -530,7 +532,7 @@ class BartStepDecoder:
                 cap = self.__dict__.get("_tree_capture_stream")
                 if cap is None:
                     cap = self._tree_capture_stream = torch.cuda.Stream(device=dev)
-                with torch.cuda.graph(g, stream=cap, capture_error_mode="thread_local"):
+                with captured(g, stream=cap, capture_error_mode="thread_local"):
                     z.hidden = forward()
                 z.graph = g
             first_of_family = st is None and not any(k[0] == "tree" and k[2:] == key[2:] for k in cache if isinstance(k, tuple))
@@ -858,7 +860,7 @@ class BartStepDecoder:
             torch.cuda.current_stream(dev).wait_stream(side)
             st.t.zero_()
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g, capture_error_mode="thread_local"):   # the aggregation thread may touch the GPU meanwhile
+            with captured(g, capture_error_mode="thread_local"):   # the aggregation thread may touch the GPU meanwhile
                 out = forward(st)
             if first:
                 st.first_logits, st.first_graph = out, g

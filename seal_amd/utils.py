@@ -1,6 +1,27 @@
 """Checkpoint loaders (reference seal/utils.py:42-50, 31-39): fairseq / lightning
-state dicts -> the HF ``BartForConditionalGeneration`` the decoder reads."""
+state dicts -> the HF ``BartForConditionalGeneration`` the decoder reads; graph capture with python's garbage collector held off."""
+import contextlib
+import gc
+
 import torch
+
+
+@contextlib.contextmanager
+def captured(graph, **kwargs):
+    """``torch.cuda.graph(graph, **kwargs)`` that no garbage collection can fall into.  A model and its step decoder refer to each other
+    (``model._seal_step_decoder``), so a decoder that is no longer used, and the graphs that it holds, go when the cyclic collector runs -- after any
+    allocation, also one made inside another graph's capture.  The destructor of a ``torch.cuda.CUDAGraph`` synchronises the device on ROCm, which
+    a capture forbids; its error leaves a destructor, and that ends the process (seen: "Fatal Python error: Aborted ... Garbage-collecting" under
+    ``tree_hidden_graph``).  So what is dead goes before the capture begins, and the collector waits until it has ended."""
+    gc.collect()
+    was = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, **kwargs):
+            yield
+    finally:
+        if was:
+            gc.enable()
 
 
 _DERIVED_KEYS = {"lm_head.weight", "final_logits_bias", "model.encoder.embed_tokens.weight", "model.decoder.embed_tokens.weight",
