@@ -16,6 +16,9 @@ SOURCES = ["fmi_host.cpp", "fmi_evidence.cpp", "fmi_agg_pack.cpp", "fmi_sdsl.cpp
 HEADERS = ["fmi_internal.h", "fmi_device.h", "fmi_agg.h", os.path.join("..", "..", "include", "sealfm.h"),
            os.path.join("..", "..", "include", "sealnn.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC"]
+# device code without packed fp32 instructions (v_pk_{add,mul,fma}_f32): hipcc -O3 forms them from ordinary float code, and some of their forms
+# have given wrong results on gfx950 now and then.  (The host pass of a .hip file says that it does not know the feature: harmless.)
+HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:
@@ -33,7 +36,7 @@ def source_digest() -> str:
     """sha256 over every source, header and the flags: what libsealfm.so must have been built from.  (mtimes say nothing about a
     git-ignored binary that travels with a snapshot: a stale library with a fresh mtime would pass an mtime check.)"""
     import hashlib
-    h = hashlib.sha256(" ".join(FLAGS).encode())
+    h = hashlib.sha256(" ".join(FLAGS + HIP_FLAGS).encode())
     for f in SOURCES + HEADERS:
         h.update(f.encode() + b"\0")
         with open(os.path.join(CSRC, f), "rb") as fh:
@@ -67,7 +70,7 @@ def stale() -> bool:
 
 def _file_digest(path: str) -> str:
     import hashlib
-    h = hashlib.sha256(" ".join(FLAGS).encode())
+    h = hashlib.sha256(" ".join(FLAGS + HIP_FLAGS).encode())
     for f in [path] + [os.path.join(CSRC, x) for x in HEADERS]:
         with open(f, "rb") as fh:
             h.update(fh.read())
@@ -93,7 +96,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         except OSError:
             have = ""
         if force or not os.path.exists(obj) or have != want:
-            cmd = [hipcc] + FLAGS + ["-c", src_path, "-o", obj]
+            cmd = [hipcc] + FLAGS + (HIP_FLAGS if src.endswith(".hip") else []) + ["-c", src_path, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
             subprocess.check_call(cmd)
