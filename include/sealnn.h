@@ -143,6 +143,57 @@ int sealnn_hgemm_nt(void *stream, const void *a, const void *w, float *c, uint32
 int sealnn_hgemm_nt_ep(void *stream, const void *a, const void *w, float *c, uint32_t M, uint32_t N, uint32_t K, uint64_t ldc, uint32_t config,
                        const float *bias, uint32_t rows_per_bias_row, float alpha);
 
+/* ---- a quantised, sampled decode (seal_amd/w4.py, kv8.py, sampling.py; fp32 and, suffix _bf16, bf16 activations) ----
+ * y [M][N] = x [M][K] (rows x_stride elements apart) W^T + bias (NULL: none), then gelu (erf form) if `gelu`.  W in 4 bits:
+ *   codes   [ceil(N / 16)][ceil(K / 128)][4 g][16 row][4 s][4] bytes: the four bytes hold the e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign)
+ *           of columns 32 s + 8 g .. + 7 of row `row` of the 16 x 128 tile, the even column in the low nibble; columns from K on are zero
+ *   scales  [ceil(N / 16)][ceil(K / 128) * 128 / group][16] bf16; group 32, 64 or 128 columns of a row
+ * fp32 x is used to its last bit (three bf16 planes), sums are fp32.  A non-finite x makes its row's products NaN. */
+int sealnn_w4_linear(void *stream, const float *x, uint64_t x_stride, const void *codes, const void *scales, const float *bias, uint32_t M, uint32_t N,
+                     uint32_t K, uint32_t group, uint32_t gelu, float *y);
+int sealnn_w4_linear_bf16(void *stream, const void *x, uint64_t x_stride, const void *codes, const void *scales, const void *bias, uint32_t M, uint32_t N,
+                          uint32_t K, uint32_t group, uint32_t gelu, void *y);
+
+/* A key / value cache of e4m3 codes with a power-of-two scale for every (slot, head, block of 16 / 32 / 64 tokens); T a multiple of 64, dh 64 or 128:
+ *   k [slots][heads][T][dh], v [slots][heads][T / 64][dh][64] (token 16 j + 4 g + r of a tile at place 16 g + 4 j + r), scales [slots][heads][T / block] fp32.
+ * Writes n new tokens of every slot (counts[slot] <= n of them if counts is given) at positions lengths[slot] ..; what would lie at T or beyond is
+ * dropped.  strides: elements between slots, tokens and heads of k_new, then of v_new (dims contiguous).  A block's scale is the smallest 2^e,
+ * e >= -64, with |x| <= 448 * 2^e for its finite new values -- and not below the scale it had if it held tokens of the slot already, whose
+ * codes are re-encoded where the scale grows.  Rounding to nearest, ties to even; infinities become +-448 * 2^e, NaN stays.  lengths is not changed. */
+int sealnn_kv8_append(void *stream, const float *k_new, const float *v_new, const uint64_t *strides, uint32_t n, const int32_t *lengths,
+                      const int32_t *counts, void *k, void *v, float *k_scale, float *v_scale, uint32_t slots, uint32_t heads, uint32_t T,
+                      uint32_t block, uint32_t dh);
+int sealnn_kv8_append_bf16(void *stream, const void *k_new, const void *v_new, const uint64_t *strides, uint32_t n, const int32_t *lengths,
+                           const int32_t *counts, void *k, void *v, float *k_scale, float *v_scale, uint32_t slots, uint32_t heads, uint32_t T,
+                           uint32_t block, uint32_t dh);
+/* out [slots * beams][heads * share][dh] = softmax(scale q K^T) V over the first lengths[slot] tokens of the row's slot (row / beams) whose
+ * keep[slot * keep_stride + token] is not 0 (keep NULL: all); nothing left: zeros.  Query head h reads cached head h / share.  splits > 1: the tokens
+ * of every slot in `splits` parts, joined by a second launch; `work` then holds slots * heads * ceil(beams * share / 16) * splits * 16 * (dh + 4) floats. */
+int sealnn_kv8_attend(void *stream, const float *q, uint64_t q_row_stride, uint64_t q_head_stride, const void *k, const void *v,
+                      const float *k_scale, const float *v_scale, const int32_t *lengths, const uint8_t *keep, uint64_t keep_stride,
+                      uint32_t slots, uint32_t beams, uint32_t heads, uint32_t share, uint32_t T, uint32_t block, uint32_t dh, float scale,
+                      uint32_t splits, void *work, uint64_t work_bytes, float *out);
+int sealnn_kv8_attend_bf16(void *stream, const void *q, uint64_t q_row_stride, uint64_t q_head_stride, const void *k, const void *v,
+                           const float *k_scale, const float *v_scale, const int32_t *lengths, const uint8_t *keep, uint64_t keep_stride,
+                           uint32_t slots, uint32_t beams, uint32_t heads, uint32_t share, uint32_t T, uint32_t block, uint32_t dh, float scale,
+                           uint32_t splits, void *work, uint64_t work_bytes, void *out);
+
+/* `draws` tokens for every row of logits [rows][vocab <= 2^18] (rows row_stride elements apart) from u [rows][draws] in [0, 1): the first token, in the order
+ * of the vocabulary, whose cumulative weight exp(logit / temperature) passes u * total, over the tokens that
+ *   bits (uint32 [rows][bits_stride], bit v of row r: token v may be drawn; NULL: all) allows, and then
+ *   are among the top_k largest (0: off; equal logits: the lower index first), then
+ *   among the fewest largest of those that hold at least top_p of their weight (>= 1: off), and
+ *   have at least min_p of the largest weight (<= 0: off).
+ * temperature <= 0: the first of the largest.  The *_v arrays ([rows], or NULL) override the numbers row by row.  NaN logits are never drawn, +inf counts as the
+ * largest fp32 number.  tokens / logprobs [rows][draws]: -1 / -inf for a row without a token; logprobs = logit - logsumexp(row), neither
+ * temperature nor filters applied. */
+int sealnn_sample_tokens(void *stream, const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float *u, uint32_t draws,
+                         const uint32_t *bits, uint64_t bits_stride, float temperature, int32_t top_k, float top_p, float min_p,
+                         const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs);
+int sealnn_sample_tokens_bf16(void *stream, const void *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float *u, uint32_t draws,
+                              const uint32_t *bits, uint64_t bits_stride, float temperature, int32_t top_k, float top_p, float min_p,
+                              const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs);
+
 #ifdef __cplusplus
 }
 #endif

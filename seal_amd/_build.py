@@ -12,8 +12,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(CSRC, "libsealfm.so")
 SOURCES = ["fmi_host.cpp", "fmi_evidence.cpp", "fmi_agg_pack.cpp", "fmi_sdsl.cpp", "fmi_kernels.hip", "fmi_aggregate.hip", "fmi_build_gpu.hip",
-           "bart_kernels.hip", "hgemm_kernels.hip", "fmi_upload.hip"]
-HEADERS = ["fmi_internal.h", "fmi_device.h", "fmi_agg.h", os.path.join("..", "..", "include", "sealfm.h"),
+           "bart_kernels.hip", "hgemm_kernels.hip", "w4_kernels.hip", "kv8_kernels.hip", "sample_kernels.hip", "fmi_upload.hip"]
+HEADERS = ["fmi_internal.h", "fmi_device.h", "fmi_agg.h", "nn_common.h", os.path.join("..", "..", "include", "sealfm.h"),
            os.path.join("..", "..", "include", "sealnn.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC"]
 # device code without packed fp32 instructions (v_pk_{add,mul,fma}_f32): hipcc -O3 forms them from ordinary float code, and some of their forms

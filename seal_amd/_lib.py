@@ -172,6 +172,13 @@ NN_SIGNATURES = {
     "sealnn_hgemm_nt": (_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u64, _u32]),
     "sealnn_hgemm_nt_ep": (_int, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u64, _u32, _vp, _u32, _f32]),
 }
+# the quantised, sampled decode: the same signatures for both storage types
+for _name, _args in (("w4_linear", [_vp, _vp, _u64, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp]),
+                     ("kv8_append", [_vp, _vp, _vp, _p64, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32]),
+                     ("kv8_attend", [_vp, _vp, _u64, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _f32,
+                                     _u32, _vp, _u64, _vp]),
+                     ("sample_tokens", [_vp, _vp, _u64, _u32, _u32, _vp, _u32, _vp, _u64, _f32, ctypes.c_int32, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _vp])):
+    NN_SIGNATURES["sealnn_" + _name] = NN_SIGNATURES["sealnn_" + _name + "_bf16"] = (_int, _args)
 
 _lib = None
 
@@ -205,6 +212,31 @@ def lib():
             raise ImportError(f"{_build.LIB}: fmi_source_digest() = {inside[:16]}, the sources present are {_build.source_digest()[:16]}: rebuild")
         _lib = L
     return _lib
+
+
+def uint64s(*values):
+    """a C array of uint64 (strides and the like)"""
+    return (_u64 * len(values))(*values)
+
+
+class launch_on:
+    """``with launch_on(tensor) as stream``: the current stream of the tensor's device (its address), that device current while the call is made"""
+    __slots__ = ("index", "old")
+
+    def __init__(self, tensor):
+        self.index = tensor.device.index
+
+    def __enter__(self):
+        import torch
+        self.old = torch.cuda.current_device()
+        if self.old != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.old != self.index:
+            import torch
+            torch.cuda.set_device(self.old)
 
 
 def check(rc: int) -> None:
