@@ -23,6 +23,12 @@ def _stream_ptr(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _pack_bits(allowed: torch.Tensor) -> torch.Tensor:
+    """bool [32 * words] -> int32 [words], bit v of word w = element 32 w + v"""
+    w = (allowed.view(-1, 32).to(torch.int64) << torch.arange(32, dtype=torch.int64)).sum(1)
+    return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
+
+
 class IndexBasedLogitsProcessor:
     """Drop-in for ``seal.beam_search.IndexBasedLogitsProcessor`` (beam_search.py:33-140)."""
 
@@ -76,10 +82,7 @@ class IndexBasedLogitsProcessor:
             allowed[torch.as_tensor(self.index.occurring_distinct, dtype=torch.long)] = True
             if self.always_allow_eos:
                 allowed[self.eos_token_id] = True
-            w = allowed.view(-1, 32).to(torch.int64) << torch.arange(32, dtype=torch.int64)
-            b = w.sum(1).to(torch.int64)
-            b = torch.where(b >= 2 ** 31, b - 2 ** 32, b).to(torch.int32).to(device)
-            cache[key] = b
+            b = cache[key] = _pack_bits(allowed).to(device)
         return b
 
     def fused_topk(self, input_ids: torch.LongTensor, logits: torch.FloatTensor, beam_scores: torch.FloatTensor,
@@ -92,6 +95,34 @@ class IndexBasedLogitsProcessor:
         range by one backward-search step instead of re-searching the prefix (same ranges)."""
         return fused_topk_groups([self], [batch], input_ids, logits, beam_scores, num_beams, parent_rows=parent_rows,
                                  tag=tag if tag is not None else ((id(self) & 0x7FFFFFFFFFFFFFFF) or 1))
+
+    def allowed_bits(self, input_ids: torch.LongTensor, vocab: int, tag: int = 0, parent_rows: Optional[torch.LongTensor] = None) -> torch.Tensor:
+        """the tokens that may follow each row of ``input_ids`` [rows, t] (the rows' own prefixes, as ``__call__`` takes them) as a bitmap: int32
+        [rows, ceil(vocab / 32)], bit v of a row set = token v is a continuation (what ``sample_tokens`` draws under).  ``tag`` / ``parent_rows``: the rows extend, by one
+        token, rows ``parent_rows`` of the previous call with this tag (one backward-search step instead of the whole prefix).  The result lives in
+        the index's workspace until the next constraint call on it."""
+        words = (vocab + 31) // 32
+        if self.forced_bos_token_id is not None:   # beam_search.py:66-71
+            if input_ids.shape[1] == 1:
+                b = torch.zeros(words * 32, dtype=torch.bool)
+                b[self.forced_bos_token_id] = True
+                return _pack_bits(b).to(input_ids.device)[None].expand(input_ids.shape[0], words)
+            input_ids, tag, parent_rows = input_ids[:, 1:], 0, None
+        if not input_ids.is_cuda:
+            raise RuntimeError("IndexBasedLogitsProcessor: the rows must live on the GPU that holds the FM-index (seal_amd has no CPU path)")
+        rows, cur_len = input_ids.shape
+        if cur_len == 1:
+            return self._first_bits(vocab, input_ids.device)[None].expand(rows, words)
+        ids = input_ids.long().contiguous()
+        ff = self.force_decoding_from or []
+        ff_arr = (ctypes.c_int64 * max(len(ff), 1))(*ff)
+        out = ctypes.c_void_p()
+        parent = parent_rows.long().contiguous() if parent_rows is not None else None
+        check(lib().fmi_dev_allowed_bits_step(
+            self.index.handle, _stream_ptr(ids.device), rows, cur_len, ids.data_ptr(), None, vocab, SHIFT, self.pad_token_id, self.eos_token_id, ff_arr, len(ff),
+            int(self.stop_at_count), int(bool(self.always_allow_eos)), int(tag), parent.data_ptr() if parent is not None else None, ctypes.byref(out)))
+        from ._lib import last_constraint_bits
+        return last_constraint_bits(self.index.handle, ids.device)
 
     def __call__(self, input_ids: torch.LongTensor, scores: torch.FloatTensor) -> torch.FloatTensor:
         if self.forced_bos_token_id is not None:   # beam_search.py:66-71
@@ -582,7 +613,8 @@ def fm_index_generate(
     if diverse_bs_groups != 1 or sample or topk or transformers_output or not keep_history:
         raise NotImplementedError(
             "seal_amd.fm_index_generate implements the SEAL search path: keep_history=True, diverse_bs_groups=1, "
-            "sample=False, topk=0 (reference retrieval.py:70-83); other modes of the reference are out of scope")
+            "sample=False, topk=0 (reference retrieval.py:70-83); other modes of the reference are out of scope "
+            "(fm_index_sample draws sequences token by token)")
     from .bart_decoder import BartStepDecoder
 
     forced_bos_token_id = kwargs.pop("forced_bos_token_id", getattr(model.config, "forced_bos_token_id", None))
@@ -622,6 +654,70 @@ def fm_index_generate(
         pg.first_logits = getattr(decoder, "first_logits", None)
         return pg
     return _history_to_hypotheses(steps, final, input_ids.shape[0], num_beams, length_penalty)
+
+
+@torch.no_grad()
+def fm_index_sample(model, index: Optional[FMIndex], input_ids: torch.LongTensor, attention_mask: torch.LongTensor, num_samples: int = 1, max_length: int = 25,
+                    temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, eos_token_id: Optional[int] = None,
+                    force_decoding_from: Optional[List[int]] = None, always_allow_eos: bool = False, disable_fm_index: bool = False,
+                    stop_at_count: int = 0, u: Optional[torch.Tensor] = None, generator: Optional[torch.Generator] = None, decoder=None,
+                    logit_bias: Optional[torch.Tensor] = None):
+    """``num_samples`` sequences for every query, drawn token by token from the model under the FM-index constraint: ``List[List[(score, token_list)]]`` like
+    ``fm_index_generate``, one list per query in the order of the draws.  (The reference's ``sample=True`` draws the 2 K candidates of a BEAM step with
+    ``torch.multinomial``, beam_search.py:296; here every sequence is a sample of its own.)
+
+    Each step is ``sample_tokens`` with the step's bitmap of allowed continuations: ``temperature``, ``top_k``, ``top_p``, ``min_p`` as there.  ``u`` fp32 [max_length - 1,
+    queries * num_samples] are the random numbers (row r of a step belongs to sample r % num_samples of query r // num_samples); by default they are drawn
+    with ``generator`` (of the input's device).  ``score`` is the sum of the model's own log-probabilities of the drawn tokens -- without temperature,
+    constraint or filters, as the beam scores are -- and ``token_list`` starts with the decoder's start token and ends with ``eos_token_id``
+    if that was drawn.  A sequence also ends where the index allows no continuation.  ``decoder``: a ``BartStepDecoder`` (default: the model's) or a
+    ``QuantStepDecoder``; ``logit_bias`` [queries, vocab] is added to the logits."""
+    from .bart_decoder import BartStepDecoder
+    from .sampling import sample_tokens
+    if num_samples < 1 or max_length < 2:
+        raise ValueError(f"fm_index_sample: num_samples = {num_samples}, max_length = {max_length}")
+    B, dev = input_ids.shape[0], input_ids.device
+    R, K = B * num_samples, num_samples
+    if u is not None and (u.dtype != torch.float32 or u.shape != (max_length - 1, R) or u.device != dev):
+        raise ValueError(f"fm_index_sample: u is fp32 {(max_length - 1, R)} on {dev}, got {u.dtype} {tuple(u.shape)} on {u.device}")
+    if decoder is None:
+        decoder = getattr(model, "_seal_step_decoder", None)
+        if decoder is None or decoder.lm_w.device != dev:
+            decoder = model._seal_step_decoder = BartStepDecoder(model)
+    cfg = model.config
+    if eos_token_id is None:
+        eos_token_id = cfg.eos_token_id
+    processor = None
+    if not disable_fm_index:
+        processor = IndexBasedLogitsProcessor(num_beams=K, index=index, pad_token_id=cfg.pad_token_id, eos_token_id=eos_token_id, force_decoding_from=force_decoding_from,
+                                              stop_at_count=stop_at_count, always_allow_eos=always_allow_eos,
+                                              forced_bos_token_id=getattr(cfg, "forced_bos_token_id", None))
+    if u is None:
+        u = torch.rand(max_length - 1, R, dtype=torch.float32, device=dev, generator=generator)
+    decoder.start(decoder.encode(input_ids, attention_mask), attention_mask, K, max_length)
+    ids = torch.full((R, max_length), cfg.pad_token_id, dtype=torch.long, device=dev)
+    ids[:, 0] = cfg.decoder_start_token_id
+    score = torch.zeros(R, dtype=torch.float32, device=dev)
+    length = torch.ones(R, dtype=torch.long, device=dev)
+    ended = torch.zeros(R, dtype=torch.bool, device=dev)
+    same, tag = torch.arange(R, device=dev), next(_LOOP_TAGS)
+    saved_bias = decoder.logit_bias
+    if logit_bias is not None:
+        decoder.logit_bias = logit_bias
+    try:
+        for t in range(1, max_length):
+            logits = decoder.step(ids[:, t - 1], beams_identical=t == 1)
+            bits = processor.allowed_bits(ids[:, :t], logits.shape[-1], tag, same) if processor is not None else None
+            tok, lp = sample_tokens(logits, u[t - 1], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, allowed_bits=bits)
+            ended = ended | (tok < 0)
+            ids[:, t] = torch.where(ended, cfg.pad_token_id, tok)
+            score = torch.where(ended, score, score + lp)
+            length = length + (~ended)
+            ended = ended | (tok == eos_token_id)
+    finally:
+        decoder.logit_bias = saved_bias
+    out = [(s, row[:n]) for s, row, n in zip(score.tolist(), ids.tolist(), length.tolist())]
+    return [out[b * K:(b + 1) * K] for b in range(B)]
 
 
 @torch.no_grad()
