@@ -12,7 +12,7 @@
 
 #include <algorithm>
 
-enum { THREADS = 1024, WAVES = THREADS / 64, STRIPE = 4 * THREADS, BUCKETS = 2048, MAX_VOCAB = 1 << 18 };
+enum { THREADS = 1024, WAVES = THREADS / 64, STRIPE = 4 * THREADS, BUCKETS = 2048, LIST = 2048, MAX_VOCAB = 1 << 18 };
 
 struct SampleArgs {
     const void *logits;
@@ -33,26 +33,31 @@ static __device__ __forceinline__ uint32_t key_of(float x) { const uint32_t u = 
 static __device__ __forceinline__ float clean(float x) { return x != x ? -__builtin_huge_valf() : fminf(x, 3.402823466e38f) + 0.f; }
 
 struct Shared {
-    uint64_t mass[BUCKETS];
+    union {
+        uint64_t mass[BUCKETS];                          // a histogram ...
+        uint64_t run[LIST];                              // ... or the running weights of the list
+    };
+    uint64_t list[LIST];                                 // (key << 32 | ~index): tokens in falling order of logit, equal ones in rising order of index
     uint64_t part[MAX_VOCAB / STRIPE * WAVES];
     uint64_t wave[WAVES];
-    float wavef[2 * WAVES];
-    double root[32];                    // 2^(i / 32)
-    uint32_t kmin, kmax, found, bucket;
-    uint64_t before, total, in_bucket;
+    float wavef[3 * WAVES];
+    double root[32];                                     // 2^(i / 32)
+    uint32_t kmin, kmax, found, bucket, n;
+    uint64_t before, total;
 };
 
-// exp((x - m) / T) * 2^44 as a whole number (0 below 2^-45)
-static __device__ __forceinline__ uint64_t weight(float x, double m, double inv_t_log2e, const double *root)
+// exp((x - m) / T) * 2^44 to nearest, as a 64-bit float (a whole number; 0 below 2^-45): 2^t = 2^floor * 2^(k / 32) * e^y, |y| <= ln 2 / 64, where the
+// series ends at y^4 (y^5 / 120 < 2^-39 relative, below the step of any weight that is not near the largest)
+static __device__ __forceinline__ double weight(float x, double m, double inv_t_log2e, const double *root)
 {
     const double t = fmax(((double)x - m) * inv_t_log2e, -64.0);
-    const double k = rint(t * 32.0);
-    const double y = (t - k * 0.03125) * 0.69314718055994530942;                      // |y| <= ln 2 / 64: the series ends at y^5 (y^6 / 720 < 2^-48)
-    const double e = 1.0 + y * (1.0 + y * (0.5 + y * (1.0 / 6 + y * (1.0 / 24 + y * (1.0 / 120)))));
-    const int ki = (int)k;
-    const double p = __hiloint2double((1023 + 44 + (ki >> 5)) << 20, 0);              // 2^(44 + floor(k / 32)), floor >= -64
-    const double v = fma(root[ki & 31] * e, p, 4503599627370496.0);                   // + 2^52: the whole number to nearest in the low bits
-    return (uint64_t)__double_as_longlong(v) & 0xfffffffffffffull;
+    const double r = t + 211106232532992.0;                                           // 1.5 * 2^47: the unit in the last place is 1 / 32
+    const double f = t - (r - 211106232532992.0);
+    const int k = __double2loint(r);                                                   // 32 t to nearest
+    const double y = f * 0.69314718055994530942;
+    const double e = 1.0 + y * (1.0 + y * (0.5 + y * (1.0 / 6 + y * (1.0 / 24))));
+    const double p = __hiloint2double((1023 + 44 + (k >> 5)) << 20, 0);               // 2^(44 + floor(k / 32))
+    return fma(root[k & 31] * e, p, 4503599627370496.0) - 4503599627370496.0;          // (+- 2^52: to the nearest whole number)
 }
 
 template <typename V> static __device__ __forceinline__ V wave_scan(V v, uint32_t lane)
@@ -73,24 +78,48 @@ static __device__ __forceinline__ uint64_t block_scan(uint64_t v, Shared &s, uin
     return v + add;
 }
 
-// The bucket (in order) at which the running sum of `value` reaches `want`: s.bucket, s.before (sum in front of it), s.in_bucket, s.total;
+// The bucket (in order) at which the running sum of s.mass reaches what is asked for: s.bucket, s.before (the sum in front of it), s.total;
 // s.found = 0 if it never does
-template <typename GET, typename REACHED>
-static __device__ __forceinline__ void find_bucket(Shared &s, uint32_t tid, uint32_t lane, uint32_t wave, GET get, REACHED reached)
+template <typename REACHED>
+static __device__ __forceinline__ void find_bucket(Shared &s, uint32_t tid, uint32_t lane, uint32_t wave, REACHED reached)
 {
     static_assert(BUCKETS == 2 * THREADS, "two buckets a thread");
-    const uint64_t a = get(2 * tid), b = get(2 * tid + 1);
+    const uint64_t a = s.mass[2 * tid], b = s.mass[2 * tid + 1];
     const uint64_t incl = block_scan(a + b, s, lane, wave);
     if (tid == 0) s.found = 0;
     if (tid == THREADS - 1) s.total = incl;
     __syncthreads();
     const uint64_t total = s.total, f0 = incl - a - b, f1 = incl - b;
-    if (!reached(f0, total) && reached(f1, total)) { s.found = 1; s.bucket = 2 * tid; s.before = f0; s.in_bucket = a; }
-    else if (!reached(f1, total) && reached(incl, total)) { s.found = 1; s.bucket = 2 * tid + 1; s.before = f1; s.in_bucket = b; }
+    if (!reached(f0, total) && reached(f1, total)) { s.found = 1; s.bucket = 2 * tid; s.before = f0; }
+    else if (!reached(f1, total) && reached(incl, total)) { s.found = 1; s.bucket = 2 * tid + 1; s.before = f1; }
     __syncthreads();
 }
 
-// One workgroup per row; every pass reads the row again.
+// s.list[0 .. n) into falling order (zeros behind it).  Up to 128 entries one wave does it alone.
+static __device__ __forceinline__ void sort_list(Shared &s, uint32_t n, uint32_t tid)
+{
+    uint32_t size = 2;
+    while (size < n) size <<= 1;
+    for (uint32_t i = n + tid; i < size; i += THREADS) s.list[i] = 0;
+    __syncthreads();
+    const bool alone = size <= 128;
+    if (!alone || tid < 64) {
+        for (uint32_t k = 2; k <= size; k <<= 1)
+            for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+                if (tid < size / 2) {
+                    const uint32_t i = ((tid & ~(j - 1)) << 1) | (tid & (j - 1)), o = i | j;
+                    const uint64_t a = s.list[i], b = s.list[o];
+                    if ((a < b) == ((i & k) == 0)) { s.list[i] = b; s.list[o] = a; }
+                }
+                if (alone) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+                else __syncthreads();
+            }
+    }
+    __syncthreads();
+}
+
+// One workgroup per row.  The row is read for the maxima and the sum of exponentials, and then once or twice more (from the caches) for what
+// the filters need; the work behind them is done on a list of the few tokens that matter, wherever there are few.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
 {
@@ -128,35 +157,41 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
         return ok & 15;
     };
     auto all = [&](auto f) {                                     // f(stripe, four logits, which may be drawn)
+#pragma unroll 2
         for (uint32_t i = 0; i < stripes; i++) { float v[4]; const uint32_t ok = fetch(i, tid, v); f(i, v, ok); }
     };
     if (tid < 32) s.root[tid] = exp2((double)tid / 32.0);
-    // the largest logit, and the largest that may be drawn
-    float mx = NINF, mz = NINF;
+    // the largest logit with the sum of exponentials (fp32: it enters the log-probabilities only), and the largest that may be drawn
+    const float L2E = 1.4426950408889634f;
+    float mx = NINF, z = 0.f, mz = NINF;
     all([&](uint32_t, const float *v, uint32_t ok) {
+        const float m4 = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), mx);
+        if (m4 > NINF) {
+            float t = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) { mx = fmaxf(mx, v[e]); mz = fmaxf(mz, (ok >> e) & 1 ? v[e] : NINF); }
+            for (int e = 0; e < 4; e++) t += __builtin_amdgcn_exp2f((v[e] - m4) * L2E);
+            z = z * __builtin_amdgcn_exp2f((mx - m4) * L2E) + t;
+            mx = m4;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) mz = fmaxf(mz, (ok >> e) & 1 ? v[e] : NINF);
     });
-    for (int o = 32; o > 0; o >>= 1) { mx = fmaxf(mx, __shfl_xor(mx, o)); mz = fmaxf(mz, __shfl_xor(mz, o)); }
-    if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; }
+    const float own_mz = mz;
+    for (int o = 32; o > 0; o >>= 1) {
+        const float om = __shfl_xor(mx, o), oz = __shfl_xor(z, o), nm = fmaxf(mx, om);
+        z = nm > NINF ? z * __builtin_amdgcn_exp2f((mx - nm) * L2E) + oz * __builtin_amdgcn_exp2f((om - nm) * L2E) : 0.f;
+        mx = nm;
+        mz = fmaxf(mz, __shfl_xor(mz, o));
+    }
+    if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; s.wavef[2 * WAVES + wave] = z; }
     __syncthreads();
     for (int w = 0; w < WAVES; w++) { mx = fmaxf(mx, s.wavef[w]); mz = fmaxf(mz, s.wavef[WAVES + w]); }
     if (mz == NINF) {                                            // nothing may be drawn
         for (uint32_t d = tid; d < a.draws; d += THREADS) { a.tokens[(uint64_t)row * a.draws + d] = -1; a.logprobs[(uint64_t)row * a.draws + d] = NINF; }
         return;
     }
-    // the log of the sum of exponentials over the whole row (fp32: it enters the log-probabilities only)
-    float z = 0.f;
-    all([&](uint32_t, const float *v, uint32_t) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) z += __builtin_amdgcn_exp2f((v[e] - mx) * 1.4426950408889634f);
-    });
-    for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o);
-    __syncthreads();
-    if (lane == 0) s.wavef[wave] = z;
-    __syncthreads();
     double zs = 0.0;
-    for (int w = 0; w < WAVES; w++) zs += (double)s.wavef[w];
+    for (int w = 0; w < WAVES; w++) zs += (double)(s.wavef[2 * WAVES + w] * __builtin_amdgcn_exp2f((s.wavef[w] - mx) * L2E));
     const double lse = (double)mx + log(zs);
 
     float temperature = a.temperature_v ? a.temperature_v[row] : a.temperature;
@@ -166,25 +201,68 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
     const double inv = 1.4426950408889634074 / (double)temperature, m = (double)mz;
     const double floor_w = min_p_ > 0.f ? (double)fminf(min_p_, 1.f) * 17592186044416.0 : 0.0;
     const float c = fminf(64.f / temperature, 1e30f);
+    // buckets of 1 / 64 of a temperature below the largest logit: they order as the logits do (a rounded difference and product are monotone)
     auto bucket0 = [&](float v) { const float b = (mz - v) * c; return b < (float)(BUCKETS - 1) ? (uint32_t)b : (uint32_t)(BUCKETS - 1); };
+    auto entry = [&](float v, uint32_t idx) { return ((uint64_t)key_of(v) << 32) | (uint32_t)~idx; };
+    auto value_of = [](uint64_t e) { const uint32_t k = (uint32_t)(e >> 32); return as_f32((k >> 31) ? k ^ 0x80000000u : ~k); };
     uint32_t thr = 0, lim = 0xffffffffu;                         // kept: key > thr, or key == thr and index <= lim
     auto kept = [&](float v, uint32_t idx) { const uint32_t k = key_of(v); return k > thr || (k == thr && idx <= lim); };
-
-    // Shortens the prefix to where the running sum of `value` reaches what `reached` asks for; `ties`(sum in front, total) = how many of the
-    // tokens that share the border's logit stay.  Members: those kept so far.
-    auto shorten = [&](auto value, auto reached, auto ties) {
+    // Tokens that satisfy `want` (of those that may be drawn) into s.list, unordered; their number (those beyond LIST are counted, not stored)
+    auto collect = [&](auto want) {
+        __syncthreads();
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        all([&](uint32_t i, const float *v, uint32_t ok) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t idx = i * STRIPE + 4 * tid + e;
+                if (((ok >> e) & 1) && want(v[e], idx)) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LIST) s.list[at] = entry(v[e], idx); }
+            }
+        });
+        __syncthreads();
+        return s.n;
+    };
+    auto clear_buckets = [&]() {
+        __syncthreads();
         for (uint32_t b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0;
         __syncthreads();
+    };
+    // running weights (or counts) of the sorted list into s.run: thread t holds entries 2 t and 2 t + 1
+    auto run_list = [&](uint32_t n, auto value) {
+        static_assert(LIST == 2 * THREADS, "two entries a thread");
+        const uint64_t w0 = 2 * tid < n ? (uint64_t)value(value_of(s.list[2 * tid])) : 0, w1 = 2 * tid + 1 < n ? (uint64_t)value(value_of(s.list[2 * tid + 1])) : 0;
+        const uint64_t incl = block_scan(w0 + w1, s, lane, wave);
+        s.run[2 * tid] = incl - w1;
+        s.run[2 * tid + 1] = incl;
+        __syncthreads();
+    };
+    // how many entries of the sorted list stand in front of the first whose running sum (plus `front`) reaches what is asked for, that one included
+    auto first_reached = [&](uint32_t n, auto reached) {
+        __syncthreads();
+        if (tid == 0) s.n = n;
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += THREADS)
+            if (reached(s.run[i]) && (i == 0 || !reached(s.run[i - 1]))) s.n = i + 1;
+        __syncthreads();
+        return s.n;
+    };
+    auto weigh = [&](float v) { return weight(v, m, inv, s.root); };
+    auto one = [](float) { return 1.0; };
+
+    // Shortens the prefix to where the running sum of `value` reaches what `reached`(sum, total) asks for: sums buckets, then orders the one bucket that the border
+    // falls into (its tokens on the list; more than the list holds -- many equal logits -- are narrowed by key, level by level).
+    auto shorten = [&](auto value, auto reached) {
+        clear_buckets();
         all([&](uint32_t i, const float *v, uint32_t ok) {
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++)
                 if (((ok >> e) & 1) && kept(v[e], i * STRIPE + 4 * tid + e)) {
-                    const uint64_t w = value(v[e]);
+                    const uint64_t w = (uint64_t)value(v[e]);
                     if (w) atomicAdd((unsigned long long *)&s.mass[bucket0(v[e])], (unsigned long long)w);
                 }
         });
         __syncthreads();
-        find_bucket(s, tid, lane, wave, [&](uint32_t b) { return s.mass[b]; }, reached);
+        find_bucket(s, tid, lane, wave, reached);
         if (!s.found) return;
         const uint32_t B = s.bucket;
         uint64_t front = s.before;
@@ -192,7 +270,17 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
         uint32_t lo = 0, hi = 0xffffffffu;                       // keys that the border lies between
         auto member = [&](float v, uint32_t idx) { const uint32_t k = key_of(v); return k >= lo && k <= hi && bucket0(v) == B && kept(v, idx); };
         for (;;) {
-            __syncthreads();
+            const uint32_t n = collect(member);
+            if (n <= LIST) {
+                sort_list(s, n, tid);
+                run_list(n, value);
+                const uint32_t stay = first_reached(n, [&](uint64_t f) { return reached(front + f, total); });
+                const uint64_t last = s.list[stay - 1];
+                thr = (uint32_t)(last >> 32);
+                lim = ~(uint32_t)last;
+                __syncthreads();
+                return;
+            }
             if (tid == 0) { s.kmin = 0xffffffffu; s.kmax = 0; }
             __syncthreads();
             uint32_t kmin = 0xffffffffu, kmax = 0;
@@ -207,29 +295,28 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
             lo = s.kmin; hi = s.kmax;
             if (lo >= hi) break;
             const uint32_t width = 32 - __clz(hi - lo), shift = width > 11 ? width - 11 : 0;
-            for (uint32_t b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0;
-            __syncthreads();
+            clear_buckets();
             all([&](uint32_t i, const float *v, uint32_t ok) {
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++)
                     if (((ok >> e) & 1) && member(v[e], i * STRIPE + 4 * tid + e))
-                        atomicAdd((unsigned long long *)&s.mass[(hi - key_of(v[e])) >> shift], (unsigned long long)value(v[e]));
+                        atomicAdd((unsigned long long *)&s.mass[(hi - key_of(v[e])) >> shift], (unsigned long long)(uint64_t)value(v[e]));
             });
             __syncthreads();
-            find_bucket(s, tid, lane, wave, [&](uint32_t b) { return s.mass[b]; }, [&](uint64_t f, uint64_t) { return reached(front + f, total); });
+            find_bucket(s, tid, lane, wave, [&](uint64_t f, uint64_t) { return reached(front + f, total); });
             if (!s.found) return;                                // (cannot be: the bucket's members sum to what the level before saw)
             front += s.before;
-            const uint32_t b = s.bucket;
-            const uint32_t top = hi - (b << shift);
+            const uint32_t top = hi - (s.bucket << shift);
             lo = max(lo, shift ? top - ((1u << shift) - 1) : top);
             hi = top;
         }
-        // one logit is left: `stay` of the tokens that have it
+        // more equal logits than the list holds: how many of them stay (each adds w), and the index of the last of those
         const uint32_t old_lim = hi == thr ? lim : 0xffffffffu;
         thr = hi;
-        const uint64_t stay = ties(front, total);
-        // the index of the last of them
-        for (uint32_t e = tid; e < stripes * WAVES; e += THREADS) s.part[e] = 0;
+        const uint64_t w = (uint64_t)value(value_of((uint64_t)thr << 32));
+        uint64_t stay = 0, step = (uint64_t)1 << 18;             // the largest number that does not reach it, plus one
+        for (; step; step >>= 1) if (!reached(front + (stay + step) * w, total)) stay += step;
+        stay++;
         __syncthreads();
         all([&](uint32_t i, const float *v, uint32_t ok) {
             uint32_t n = 0;
@@ -262,34 +349,77 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
         lim = at != 0xffffffffu ? min(old_lim, s.bucket) : old_lim;
         __syncthreads();
     };
+    // (a prefix of mass f is long enough; an empty one never is)
+    const double p = (double)fmaxf(top_p, 0.f);
+    auto enough = [&](uint64_t f, uint64_t total) { return f > 0 && (double)f >= p * (double)total; };
+    uint32_t listed = 0;                                         // > 0: the kept tokens, and no others, are the first `listed` of the sorted list
     if (top_k > 0 && (uint32_t)top_k < V) {
         const uint64_t k = (uint64_t)top_k;
-        shorten([&](float) { return (uint64_t)1; }, [&](uint64_t f, uint64_t) { return f >= k; }, [&](uint64_t front, uint64_t) { return k - front; });
+        // k of the threads' largest logits are at least as large as what bucket B holds: so are the k largest of the row
+        uint32_t n = LIST + 1;
+        if (k <= THREADS / 2) {
+            clear_buckets();
+            if (own_mz > NINF) atomicAdd((unsigned long long *)&s.mass[bucket0(own_mz)], 1ull);
+            __syncthreads();
+            find_bucket(s, tid, lane, wave, [&](uint64_t f, uint64_t) { return f >= k; });
+            const uint32_t B = s.found ? s.bucket : BUCKETS - 1;
+            n = collect([&](float v, uint32_t) { return bucket0(v) <= B; });
+        }
+        if (n <= LIST) {
+            sort_list(s, n, tid);
+            listed = min(n, (uint32_t)k);
+        } else {
+            shorten(one, [&](uint64_t f, uint64_t) { return f >= k; });
+        }
     }
     if (top_p < 1.f) {
-        const double p = (double)fmaxf(top_p, 0.f);
-        // (a prefix of mass f is long enough; an empty one never is)
-        auto enough = [&](uint64_t f, uint64_t total) { return f > 0 && (double)f >= p * (double)total; };
-        shorten([&](float v) { return weight(v, m, inv, s.root); }, enough, [&](uint64_t front, uint64_t total) {
-            const uint64_t w = weight(as_f32((thr >> 31) ? thr ^ 0x80000000u : ~thr), m, inv, s.root);
-            uint64_t n = (uint64_t)fmax(1.0, ceil((p * (double)total - (double)front) / (double)w));
-            while (n > 1 && enough(front + (n - 1) * w, total)) n--;
-            while (!enough(front + n * w, total)) n++;
-            return n;
-        });
+        if (listed) {
+            run_list(listed, weigh);
+            const uint64_t total = s.run[listed - 1];
+            listed = first_reached(listed, [&](uint64_t f) { return enough(f, total); });
+        } else {
+            shorten(weigh, enough);
+        }
     }
-    // the weights of what is left, summed for every 256 tokens
-    auto final_weight = [&](float v, uint32_t idx, uint32_t ok) -> uint64_t {
-        if (!ok || !kept(v, idx)) return 0;
-        const uint64_t w = weight(v, m, inv, s.root);
-        return (double)w >= floor_w ? w : 0;
+    // a draw's place in the running weights: floor(u * total)
+    auto target_of = [&](uint32_t d, uint64_t total) {
+        const float u = a.u[(uint64_t)row * a.draws + d];
+        const double uc = u > 0.f ? fmin((double)u, 1.0 - 1.0 / 16777216) : 0.0;
+        const uint64_t u63 = (uint64_t)(uc * 9223372036854775808.0);
+        return (__umul64hi(u63, total) << 1) | ((u63 * total) >> 63);
     };
+    auto put = [&](uint32_t d, uint32_t idx, float v) {
+        a.tokens[(uint64_t)row * a.draws + d] = idx;
+        a.logprobs[(uint64_t)row * a.draws + d] = (float)((double)v - lse);
+    };
+    auto floored = [&](float v) { const double w = weigh(v); return w >= floor_w ? w : 0.0; };
+    if (listed) {
+        // into the order of the vocabulary: (~index << 32 | key) falls as the index rises
+        __syncthreads();
+        for (uint32_t i = tid; i < listed; i += THREADS) s.list[i] = (s.list[i] << 32) | (s.list[i] >> 32);
+        sort_list(s, listed, tid);
+        for (uint32_t i = tid; i < listed; i += THREADS) s.list[i] = (s.list[i] << 32) | (s.list[i] >> 32);
+        __syncthreads();
+        run_list(listed, floored);
+        const uint64_t total = s.run[listed - 1];
+        for (uint32_t d = tid; d < a.draws; d += THREADS) {
+            const uint64_t target = target_of(d, total);
+            uint32_t lo = 0, hi = listed - 1;
+            while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (s.run[mid] > target) hi = mid; else lo = mid + 1; }
+            put(d, ~(uint32_t)s.list[lo], value_of(s.list[lo]));
+        }
+        return;
+    }
+    // the weights of what is left, summed for every 256 tokens (a logit below `reach` has none: less than min_p of the largest weight, or 2^-45)
+    const float reach = mz - temperature * fminf(31.5f, floor_w > 0.0 ? 1e-3f - 0.69314718f * __builtin_amdgcn_logf(fminf(min_p_, 1.f)) : 31.5f) * 1.00001f;
+    auto final_weight = [&](float v, uint32_t idx, uint32_t ok) -> uint64_t { return ok && !(v < reach) && kept(v, idx) ? (uint64_t)floored(v) : 0; };
     __syncthreads();
     all([&](uint32_t i, const float *v, uint32_t ok) {
         uint64_t w = 0;
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++) w += final_weight(v[e], i * STRIPE + 4 * tid + e, (ok >> e) & 1);
-        for (int o = 32; o > 0; o >>= 1) w += __shfl_xor(w, o);
+        if (__any(w != 0))
+            for (int o = 32; o > 0; o >>= 1) w += __shfl_xor(w, o);
         if (lane == 0) s.part[i * WAVES + wave] = w;
     });
     __syncthreads();
@@ -299,10 +429,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
     __syncthreads();
     const uint64_t total = s.part[parts - 1];
     for (uint32_t d = wave; d < a.draws; d += WAVES) {
-        const float u = a.u[(uint64_t)row * a.draws + d];
-        const double uc = u > 0.f ? fmin((double)u, 1.0 - 1.0 / 16777216) : 0.0;
-        const uint64_t u63 = (uint64_t)(uc * 9223372036854775808.0);
-        const uint64_t target = (__umul64hi(u63, total) << 1) | ((u63 * total) >> 63);      // floor(u * total)
+        const uint64_t target = target_of(d, total);
         uint32_t lo = 0, hi = parts - 1;                         // the first part whose running sum passes the target
         while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (s.part[mid] > target) hi = mid; else lo = mid + 1; }
         const uint64_t rest = target - (lo ? s.part[lo - 1] : 0);
@@ -318,11 +445,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) {
                 run += w[e];
-                if (!done && run > rest) {
-                    done = true;
-                    a.tokens[(uint64_t)row * a.draws + d] = idx + e;
-                    a.logprobs[(uint64_t)row * a.draws + d] = (float)((double)v[e] - lse);
-                }
+                if (!done && run > rest) { done = true; put(d, idx + e, v[e]); }
             }
         }
     }
