@@ -28,21 +28,20 @@ struct SampleArgs {
     float *logprobs;
 };
 
-static __device__ __forceinline__ uint32_t key_of(float x) { const uint32_t u = as_u32(x); return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u); }
-// NaN counts as -inf, +inf as the largest number, -0 as +0
-static __device__ __forceinline__ float clean(float x) { return x != x ? -__builtin_huge_valf() : fminf(x, 3.402823466e38f) + 0.f; }
+// monotone in x; +0 and -0 alike
+static __device__ __forceinline__ uint32_t key_of(float x) { const uint32_t u = as_u32(x + 0.f); return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u); }
+// NaN counts as -inf, +inf as the largest number (the larger of NaN and a number is the number)
+static __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -__builtin_huge_valf()), 3.402823466e38f); }
 
 struct Shared {
-    union {
-        uint64_t mass[BUCKETS];                          // a histogram ...
-        uint64_t run[LIST];                              // ... or the running weights of the list
-    };
-    uint64_t list[LIST];                                 // (key << 32 | ~index): tokens in falling order of logit, equal ones in rising order of index
-    uint64_t part[MAX_VOCAB / STRIPE * WAVES];
+    uint64_t mass[BUCKETS];                              // a histogram, or the running weights of `order`
+    uint64_t list[LIST];                                 // (key << 32 | ~index) of the tokens that matter: falling order = falling logit, equal ones by rising index
+    uint64_t order[LIST];                                // those of them that a border falls between
+    uint64_t part[MAX_VOCAB / 256];                      // weights of 256 consecutive tokens each
     uint64_t wave[WAVES];
-    float wavef[3 * WAVES];
+    float wavef[2 * WAVES];
     double root[32];                                     // 2^(i / 32)
-    uint32_t kmin, kmax, found, bucket, n;
+    uint32_t kmin, kmax, found, bucket, n, thr, lim;
     uint64_t before, total;
 };
 
@@ -60,22 +59,44 @@ static __device__ __forceinline__ double weight(float x, double m, double inv_t_
     return fma(root[k & 31] * e, p, 4503599627370496.0) - 4503599627370496.0;          // (+- 2^52: to the nearest whole number)
 }
 
-template <typename V> static __device__ __forceinline__ V wave_scan(V v, uint32_t lane)
+// DPP: the value of another lane of the wave without a trip through LDS (lanes that have none get `none`)
+template <int CTRL, int ROWS> static __device__ __forceinline__ uint32_t dpp(uint32_t none, uint32_t v)
+{ return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS> static __device__ __forceinline__ uint64_t dpp_add(uint64_t v)
+{ return v + (((uint64_t)dpp<CTRL, ROWS>(0, (uint32_t)(v >> 32)) << 32) | dpp<CTRL, ROWS>(0, (uint32_t)v)); }
+// inclusive sums over the wave: within rows of 16 lanes, then the rows' last lanes onwards
+static __device__ __forceinline__ uint64_t wave_scan(uint64_t v)
 {
-    for (uint32_t o = 1; o < 64; o <<= 1) { const V w = __shfl_up(v, o); if (lane >= o) v += w; }
-    return v;
+    v = dpp_add<0x111, 0xf>(v); v = dpp_add<0x112, 0xf>(v); v = dpp_add<0x114, 0xf>(v); v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    return dpp_add<0x143, 0xc>(v);
+}
+static __device__ __forceinline__ uint64_t wave_total(uint64_t scanned)
+{
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(scanned >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)scanned, 63);
+}
+template <int CTRL, int ROWS> static __device__ __forceinline__ float dpp_max(float v)
+{ return fmaxf(v, as_f32(dpp<CTRL, ROWS>(0xff800000u, as_u32(v)))); }
+static __device__ __forceinline__ float wave_max(float v)
+{
+    v = dpp_max<0x111, 0xf>(v); v = dpp_max<0x112, 0xf>(v); v = dpp_max<0x114, 0xf>(v); v = dpp_max<0x118, 0xf>(v);
+    v = dpp_max<0x142, 0xa>(v);
+    v = dpp_max<0x143, 0xc>(v);
+    return as_f32((uint32_t)__builtin_amdgcn_readlane((int)as_u32(v), 63));
 }
 
-// inclusive sums over the workgroup
-static __device__ __forceinline__ uint64_t block_scan(uint64_t v, Shared &s, uint32_t lane, uint32_t wave)
+// inclusive sums over the workgroup; `total` the whole sum
+static __device__ __forceinline__ uint64_t block_scan(uint64_t v, Shared &s, uint32_t lane, uint32_t wave, uint64_t &total)
 {
-    v = wave_scan(v, lane);
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) s.wave[wave] = v;
     __syncthreads();
-    uint64_t add = 0;
-    for (uint32_t w = 0; w < wave; w++) add += s.wave[w];
-    return v + add;
+    const uint64_t w = wave_scan(lane < WAVES ? s.wave[lane] : 0);
+    total = wave_total(w);
+    const uint64_t before = wave ? (((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), (int)(wave - 1)) << 32) |
+                                    (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)w, (int)(wave - 1))) : 0;
+    return v + before;
 }
 
 // The bucket (in order) at which the running sum of s.mass reaches what is asked for: s.bucket, s.before (the sum in front of it), s.total;
@@ -85,210 +106,236 @@ static __device__ __forceinline__ void find_bucket(Shared &s, uint32_t tid, uint
 {
     static_assert(BUCKETS == 2 * THREADS, "two buckets a thread");
     const uint64_t a = s.mass[2 * tid], b = s.mass[2 * tid + 1];
-    const uint64_t incl = block_scan(a + b, s, lane, wave);
-    if (tid == 0) s.found = 0;
-    if (tid == THREADS - 1) s.total = incl;
+    uint64_t total;
+    const uint64_t incl = block_scan(a + b, s, lane, wave, total);
+    if (tid == 0) { s.found = 0; s.total = total; }
     __syncthreads();
-    const uint64_t total = s.total, f0 = incl - a - b, f1 = incl - b;
+    const uint64_t f0 = incl - a - b, f1 = incl - b;
     if (!reached(f0, total) && reached(f1, total)) { s.found = 1; s.bucket = 2 * tid; s.before = f0; }
     else if (!reached(f1, total) && reached(incl, total)) { s.found = 1; s.bucket = 2 * tid + 1; s.before = f1; }
     __syncthreads();
 }
 
-// s.list[0 .. n) into falling order (zeros behind it).  Up to 128 entries one wave does it alone.
-static __device__ __forceinline__ void sort_list(Shared &s, uint32_t n, uint32_t tid)
+// s.order[0 .. n) into falling order (zeros behind it)
+static __device__ __forceinline__ void sort_order(Shared &s, uint32_t n, uint32_t tid)
 {
     uint32_t size = 2;
     while (size < n) size <<= 1;
-    for (uint32_t i = n + tid; i < size; i += THREADS) s.list[i] = 0;
+    for (uint32_t i = n + tid; i < size; i += THREADS) s.order[i] = 0;
     __syncthreads();
-    const bool alone = size <= 128;
-    if (!alone || tid < 64) {
-        for (uint32_t k = 2; k <= size; k <<= 1)
-            for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-                if (tid < size / 2) {
-                    const uint32_t i = ((tid & ~(j - 1)) << 1) | (tid & (j - 1)), o = i | j;
-                    const uint64_t a = s.list[i], b = s.list[o];
-                    if ((a < b) == ((i & k) == 0)) { s.list[i] = b; s.list[o] = a; }
-                }
-                if (alone) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-                else __syncthreads();
+    for (uint32_t k = 2; k <= size; k <<= 1)
+        for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+            if (tid < size / 2) {
+                const uint32_t i = ((tid & ~(j - 1)) << 1) | (tid & (j - 1)), o = i | j;
+                const uint64_t a = s.order[i], b = s.order[o];
+                if ((a < b) == ((i & k) == 0)) { s.order[i] = b; s.order[o] = a; }
             }
-    }
-    __syncthreads();
+            __syncthreads();
+        }
+}
+// a value per lane of one wave into falling order
+static __device__ __forceinline__ uint64_t sort_wave(uint64_t v, uint32_t lane)
+{
+#pragma unroll
+    for (uint32_t k = 2; k <= 64; k <<= 1)
+#pragma unroll
+        for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+            const uint64_t o = __shfl_xor(v, (int)j);
+            const bool larger = ((lane & k) == 0) == ((lane & j) == 0);                // this lane keeps the larger of the two
+            v = (o > v) == larger ? o : v;
+        }
+    return v;
 }
 
-// One workgroup per row.  The row is read for the maxima and the sum of exponentials, and then once or twice more (from the caches) for what
-// the filters need; the work behind them is done on a list of the few tokens that matter, wherever there are few.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
+// One workgroup per row.  The row is read for the maxima, then once more (from the caches): for the sum of exponentials, the weights where a nucleus needs
+// their total, and a list of the largest tokens -- those that reach the k-th largest (top-k) or the 768th largest (a nucleus) of the threads' own
+// maxima.  Where the list holds what the filters leave, everything else happens on it; otherwise the filters read the row again.
+template <typename T, bool BITS>
+__global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
 {
     __shared__ Shared s;
     const float NINF = -__builtin_huge_valf();
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, V = a.vocab;
     const T *x = (const T *)a.logits + (uint64_t)row * a.row_stride;
-    const uint32_t *bits = a.bits ? a.bits + (uint64_t)row * a.bits_stride : nullptr;
+    const uint32_t *bits = BITS ? a.bits + (uint64_t)row * a.bits_stride : nullptr;
     const uint32_t stripes = (V + STRIPE - 1) / STRIPE;
-    // four logits of stripe i (-inf beyond the row) and which of them may be drawn
-    auto fetch = [&](uint32_t i, uint32_t t, float v[4]) -> uint32_t {
-        const uint32_t at = i * STRIPE + 4 * t;
-        uint32_t ok = 0;
-        if (at + 4 <= V) {
-            if constexpr (std::is_same<T, float>::value) {
-                const f32x4_a4 w = *(const f32x4_a4 *)(x + at);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = w[e];
-            } else {
-                const u16x4_a2 w = *(const u16x4_a2 *)(x + at);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = as_f32((uint32_t)w[e] << 16);
-            }
-            ok = 15;
+    // Four logits of stripe i as they lie in memory, without a branch: lanes that reach over the end of the row read its last four (a row of less
+    // than four its first, again and again), and `unpack` moves them into place -- so that several stripes' loads are in flight at once
+    typedef typename std::conditional<std::is_same<T, float>::value, f32x4, u32x2>::type Raw;
+    auto load = [&](uint32_t i, uint32_t t) -> Raw {
+        const uint32_t at = min(i * STRIPE + 4 * t, V < 4 ? 0 : V - 4);
+        if constexpr (std::is_same<T, float>::value) {
+            if (V >= 4) { const f32x4_a4 w = *(const f32x4_a4 *)(x + at); return f32x4{w[0], w[1], w[2], w[3]}; }
+            return f32x4{x[0], x[min(1u, V - 1)], x[min(2u, V - 1)], NINF};
         } else {
+            const uint16_t *h = (const uint16_t *)x;
+            if (V >= 4) { const u16x4_a2 w = *(const u16x4_a2 *)(h + at); return __builtin_bit_cast(u32x2, w); }
+            return u32x2{(uint32_t)h[0] | ((uint32_t)h[min(1u, V - 1)] << 16), (uint32_t)h[min(2u, V - 1)]};
+        }
+    };
+    auto load_bits = [&](uint32_t i, uint32_t t) -> uint32_t { return BITS ? bits[min(i * STRIPE + 4 * t, V - 1) >> 5] : 0; };
+    // the logits as they are (-inf beyond the row); returns which of them may be drawn
+    auto unpack = [&](uint32_t i, uint32_t t, Raw w, uint32_t word, float v[4]) -> uint32_t {
+        const uint32_t at = i * STRIPE + 4 * t;
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) {
-                v[e] = at + e < V ? load1(x + at + e) : NINF;
-                ok |= at + e < V ? 1u << e : 0u;
+        for (int e = 0; e < 4; e++) {
+            if constexpr (std::is_same<T, float>::value) v[e] = w[e];
+            else v[e] = as_f32(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        }
+        if (i == stripes - 1) {
+            if (V >= 4 && at + 4 > V) {
+                const uint32_t skip = at + 4 - V;
+                v[0] = skip == 1 ? v[1] : skip == 2 ? v[2] : skip == 3 ? v[3] : NINF;
+                v[1] = skip == 1 ? v[2] : skip == 2 ? v[3] : NINF;
+                v[2] = skip == 1 ? v[3] : NINF;
+                v[3] = NINF;
+            }
+            if (V < 4) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) if (at + e >= V) v[e] = NINF;
             }
         }
-        if (bits && at < V) ok &= bits[at >> 5] >> (at & 31);
-#pragma unroll
-        for (int e = 0; e < 4; e++) { v[e] = clean(v[e]); if (v[e] == NINF) ok &= ~(1u << e); }
-        return ok & 15;
+        return BITS ? (word >> (at & 31)) & 15u : 15u;
     };
-    auto all = [&](auto f) {                                     // f(stripe, four logits, which may be drawn)
-#pragma unroll 2
-        for (uint32_t i = 0; i < stripes; i++) { float v[4]; const uint32_t ok = fetch(i, tid, v); f(i, v, ok); }
+    auto row_pass = [&](auto f) {                                // f(index of the first, four logits, which may be drawn)
+        enum { FLY = 4 };
+        for (uint32_t i0 = 0; i0 < stripes; i0 += FLY) {
+            Raw w[FLY];
+            uint32_t b[FLY];
+#pragma unroll
+            for (uint32_t j = 0; j < FLY; j++) { const uint32_t i = min(i0 + j, stripes - 1); w[j] = load(i, tid); b[j] = load_bits(i, tid); }
+#pragma unroll
+            for (uint32_t j = 0; j < FLY; j++)
+                if (i0 + j < stripes) { float v[4]; const uint32_t ok = unpack(i0 + j, tid, w[j], b[j], v); f((i0 + j) * STRIPE + 4 * tid, v, ok); }
+        }
     };
     if (tid < 32) s.root[tid] = exp2((double)tid / 32.0);
-    // the largest logit with the sum of exponentials (fp32: it enters the log-probabilities only), and the largest that may be drawn
+    // the largest logit, and the largest that may be drawn (fmaxf leaves NaN out)
     const float L2E = 1.4426950408889634f;
-    float mx = NINF, z = 0.f, mz = NINF;
-    all([&](uint32_t, const float *v, uint32_t ok) {
-        const float m4 = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), mx);
-        if (m4 > NINF) {
-            float t = 0.f;
+    float mx = NINF, mz = NINF;
+    row_pass([&](uint32_t, const float *v, uint32_t ok) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) t += __builtin_amdgcn_exp2f((v[e] - m4) * L2E);
-            z = z * __builtin_amdgcn_exp2f((mx - m4) * L2E) + t;
-            mx = m4;
+        for (int e = 0; e < 4; e++) {
+            mx = fmaxf(mx, v[e]);
+            if (BITS) mz = fmaxf(mz, (ok >> e) & 1 ? v[e] : NINF);
         }
-#pragma unroll
-        for (int e = 0; e < 4; e++) mz = fmaxf(mz, (ok >> e) & 1 ? v[e] : NINF);
     });
-    const float own_mz = mz;
-    for (int o = 32; o > 0; o >>= 1) {
-        const float om = __shfl_xor(mx, o), oz = __shfl_xor(z, o), nm = fmaxf(mx, om);
-        z = nm > NINF ? z * __builtin_amdgcn_exp2f((mx - nm) * L2E) + oz * __builtin_amdgcn_exp2f((om - nm) * L2E) : 0.f;
-        mx = nm;
-        mz = fmaxf(mz, __shfl_xor(mz, o));
-    }
-    if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; s.wavef[2 * WAVES + wave] = z; }
+    const float own = clean(BITS ? mz : mx);                     // the thread's own
+    mx = wave_max(mx);
+    mz = BITS ? wave_max(mz) : mx;
+    if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; }
     __syncthreads();
-    for (int w = 0; w < WAVES; w++) { mx = fmaxf(mx, s.wavef[w]); mz = fmaxf(mz, s.wavef[WAVES + w]); }
+    mx = clean(wave_max(s.wavef[lane % WAVES]));
+    mz = clean(wave_max(s.wavef[WAVES + lane % WAVES]));
     if (mz == NINF) {                                            // nothing may be drawn
         for (uint32_t d = tid; d < a.draws; d += THREADS) { a.tokens[(uint64_t)row * a.draws + d] = -1; a.logprobs[(uint64_t)row * a.draws + d] = NINF; }
         return;
     }
-    double zs = 0.0;
-    for (int w = 0; w < WAVES; w++) zs += (double)(s.wavef[2 * WAVES + w] * __builtin_amdgcn_exp2f((s.wavef[w] - mx) * L2E));
-    const double lse = (double)mx + log(zs);
-
     float temperature = a.temperature_v ? a.temperature_v[row] : a.temperature;
     int32_t top_k = a.top_k_v ? a.top_k_v[row] : a.top_k;
-    const float top_p = a.top_p_v ? a.top_p_v[row] : a.top_p, min_p_ = a.min_p_v ? a.min_p_v[row] : a.min_p;
+    const float top_p = a.top_p_v ? a.top_p_v[row] : a.top_p;
+    float min_p = a.min_p_v ? a.min_p_v[row] : a.min_p;
+    min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
     if (!(temperature > 0.f)) { temperature = 1.f; top_k = 1; }                       // greedy: the first of the largest
     const double inv = 1.4426950408889634074 / (double)temperature, m = (double)mz;
-    const double floor_w = min_p_ > 0.f ? (double)fminf(min_p_, 1.f) * 17592186044416.0 : 0.0;
-    const float c = fminf(64.f / temperature, 1e30f);
+    auto weigh = [&](float v) { return weight(v, m, inv, s.root); };
+    auto one = [](float) { return 1.0; };
     // buckets of 1 / 64 of a temperature below the largest logit: they order as the logits do (a rounded difference and product are monotone)
+    const float c = fminf(64.f / temperature, 1e30f);
     auto bucket0 = [&](float v) { const float b = (mz - v) * c; return b < (float)(BUCKETS - 1) ? (uint32_t)b : (uint32_t)(BUCKETS - 1); };
-    auto entry = [&](float v, uint32_t idx) { return ((uint64_t)key_of(v) << 32) | (uint32_t)~idx; };
     auto value_of = [](uint64_t e) { const uint32_t k = (uint32_t)(e >> 32); return as_f32((k >> 31) ? k ^ 0x80000000u : ~k); };
     uint32_t thr = 0, lim = 0xffffffffu;                         // kept: key > thr, or key == thr and index <= lim
     auto kept = [&](float v, uint32_t idx) { const uint32_t k = key_of(v); return k > thr || (k == thr && idx <= lim); };
-    // Tokens that satisfy `want` (of those that may be drawn) into s.list, unordered; their number (those beyond LIST are counted, not stored)
-    auto collect = [&](auto want) {
-        __syncthreads();
-        if (tid == 0) s.n = 0;
-        __syncthreads();
-        all([&](uint32_t i, const float *v, uint32_t ok) {
+    // The sum of exponentials over the whole row (fp32: it enters the log-probabilities only), added up by the first pass behind the maxima; v cleaned
+    float z = 0.f;
+    bool have_z = false;
+    auto add_z = [&](const float *v) {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) {
-                const uint32_t idx = i * STRIPE + 4 * tid + e;
-                if (((ok >> e) & 1) && want(v[e], idx)) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LIST) s.list[at] = entry(v[e], idx); }
+        for (int e = 0; e < 4; e++) z += __builtin_amdgcn_exp2f((v[e] - mx) * L2E);
+    };
+    // every token that may be drawn and is at least `from`: f(cleaned logit, index); also(four cleaned logits, which may be drawn)
+    auto row_from = [&](float from, auto f, auto also) {
+        row_pass([&](uint32_t at, float *v, uint32_t ok) {
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) { v[e] = clean(v[e]); any |= v[e] >= from; }
+            also(v, ok);
+            if (any) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) if (v[e] >= from && (!BITS || ((ok >> e) & 1))) f(v[e], at + e);
             }
         });
-        __syncthreads();
-        return s.n;
     };
+    const float LOWEST = -3.402823466e38f;                       // (a logit of -inf is never drawn)
+    auto nothing = [](const float *, uint32_t) {};
     auto clear_buckets = [&]() {
         __syncthreads();
-        for (uint32_t b = tid; b < BUCKETS; b += THREADS) s.mass[b] = 0;
+        s.mass[tid] = s.mass[tid + THREADS] = 0;
+        if (tid == 0) s.n = 0;
         __syncthreads();
     };
-    // running weights (or counts) of the sorted list into s.run: thread t holds entries 2 t and 2 t + 1
-    auto run_list = [&](uint32_t n, auto value) {
-        static_assert(LIST == 2 * THREADS, "two entries a thread");
-        const uint64_t w0 = 2 * tid < n ? (uint64_t)value(value_of(s.list[2 * tid])) : 0, w1 = 2 * tid + 1 < n ? (uint64_t)value(value_of(s.list[2 * tid + 1])) : 0;
-        const uint64_t incl = block_scan(w0 + w1, s, lane, wave);
-        s.run[2 * tid] = incl - w1;
-        s.run[2 * tid + 1] = incl;
-        __syncthreads();
-    };
-    // how many entries of the sorted list stand in front of the first whose running sum (plus `front`) reaches what is asked for, that one included
-    auto first_reached = [&](uint32_t n, auto reached) {
-        __syncthreads();
-        if (tid == 0) s.n = n;
-        __syncthreads();
-        for (uint32_t i = tid; i < n; i += THREADS)
-            if (reached(s.run[i]) && (i == 0 || !reached(s.run[i - 1]))) s.n = i + 1;
-        __syncthreads();
-        return s.n;
-    };
-    auto weigh = [&](float v) { return weight(v, m, inv, s.root); };
-    auto one = [](float) { return 1.0; };
+    uint32_t listed = 0;                                         // > 0: everything that is kept is among the list's first entries (in no order)
+    auto list_pass = [&](auto f) { for (uint32_t i = tid; i < listed; i += THREADS) f(value_of(s.list[i]), ~(uint32_t)s.list[i]); };
+    auto put_order = [&](float v, uint32_t idx) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LIST) s.order[at] = ((uint64_t)key_of(v) << 32) | (uint32_t)~idx; };
 
-    // Shortens the prefix to where the running sum of `value` reaches what `reached`(sum, total) asks for: sums buckets, then orders the one bucket that the border
-    // falls into (its tokens on the list; more than the list holds -- many equal logits -- are narrowed by key, level by level).
-    auto shorten = [&](auto value, auto reached) {
+    // The border inside s.order[0 .. n), all of it kept so far, behind a sum of `front`: thr and lim become the first token (in order) whose running sum
+    // of `value` reaches what is asked for.  Up to 64 tokens one wave sorts in registers.
+    auto border = [&](uint32_t n, uint64_t front, auto value, auto reached) {
+        if (n <= 64) {
+            if (wave == 0) {
+                const uint64_t e = sort_wave(lane < n ? s.order[lane] : 0, lane);
+                const uint64_t run = front + wave_scan(lane < n ? (uint64_t)value(value_of(e)) : 0);
+                const uint64_t hit = __ballot(lane < n && reached(run));
+                const uint32_t first = hit ? (uint32_t)__ffsll((unsigned long long)hit) - 1 : n - 1;
+                if (lane == first) { s.thr = (uint32_t)(e >> 32); s.lim = ~(uint32_t)e; }
+            }
+        } else {
+            sort_order(s, n, tid);
+            const uint64_t w0 = 2 * tid < n ? (uint64_t)value(value_of(s.order[2 * tid])) : 0, w1 = 2 * tid + 1 < n ? (uint64_t)value(value_of(s.order[2 * tid + 1])) : 0;
+            uint64_t sum;
+            const uint64_t incl = front + block_scan(w0 + w1, s, lane, wave, sum);
+            // (the running sums grow: one thread finds the first that reaches it, or the last entry stands)
+            const bool r0 = reached(incl - w1), r1 = reached(incl), before = 2 * tid > 0 && reached(incl - w0 - w1);
+            const uint32_t at = r0 ? 2 * tid : 2 * tid + 1;
+            if (tid == 0) { s.thr = (uint32_t)(s.order[n - 1] >> 32); s.lim = ~(uint32_t)s.order[n - 1]; }
+            __syncthreads();
+            if ((r0 || r1) && !before && at < n) { s.thr = (uint32_t)(s.order[at] >> 32); s.lim = ~(uint32_t)s.order[at]; }
+        }
+        __syncthreads();
+        thr = s.thr;
+        lim = s.lim;
+        __syncthreads();
+    };
+    // Shortens the prefix to where the running sum of `value` over the kept tokens reaches what is asked for (false: it never does; nothing changes): sums buckets,
+    // then orders the one bucket that the border falls into.  `pass` goes over the list or the row.
+    auto shorten = [&](auto pass, auto value, auto reached) -> bool {
         clear_buckets();
-        all([&](uint32_t i, const float *v, uint32_t ok) {
-#pragma unroll
-            for (uint32_t e = 0; e < 4; e++)
-                if (((ok >> e) & 1) && kept(v[e], i * STRIPE + 4 * tid + e)) {
-                    const uint64_t w = (uint64_t)value(v[e]);
-                    if (w) atomicAdd((unsigned long long *)&s.mass[bucket0(v[e])], (unsigned long long)w);
-                }
+        pass([&](float v, uint32_t idx) {
+            if (!kept(v, idx)) return;
+            const uint64_t w = (uint64_t)value(v);
+            if (w) atomicAdd((unsigned long long *)&s.mass[bucket0(v)], (unsigned long long)w);
         });
         __syncthreads();
-        find_bucket(s, tid, lane, wave, reached);
-        if (!s.found) return;
+        find_bucket(s, tid, lane, wave, [&](uint64_t f, uint64_t) { return reached(f); });
+        if (!s.found) return false;
         const uint32_t B = s.bucket;
         uint64_t front = s.before;
-        const uint64_t total = s.total;
         uint32_t lo = 0, hi = 0xffffffffu;                       // keys that the border lies between
         auto member = [&](float v, uint32_t idx) { const uint32_t k = key_of(v); return k >= lo && k <= hi && bucket0(v) == B && kept(v, idx); };
         for (;;) {
-            const uint32_t n = collect(member);
-            if (n <= LIST) {
-                sort_list(s, n, tid);
-                run_list(n, value);
-                const uint32_t stay = first_reached(n, [&](uint64_t f) { return reached(front + f, total); });
-                const uint64_t last = s.list[stay - 1];
-                thr = (uint32_t)(last >> 32);
-                lim = ~(uint32_t)last;
-                __syncthreads();
-                return;
-            }
-            if (tid == 0) { s.kmin = 0xffffffffu; s.kmax = 0; }
             __syncthreads();
+            if (tid == 0) { s.n = 0; s.kmin = 0xffffffffu; s.kmax = 0; }
+            __syncthreads();
+            pass([&](float v, uint32_t idx) { if (member(v, idx)) put_order(v, idx); });
+            __syncthreads();
+            const uint32_t n = s.n;
+            if (n <= LIST) {
+                border(n, front, value, reached);
+                return true;
+            }
+            // more than can be sorted (many equal logits): narrowed by key, level by level
             uint32_t kmin = 0xffffffffu, kmax = 0;
-            all([&](uint32_t i, const float *v, uint32_t ok) {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e++)
-                    if (((ok >> e) & 1) && member(v[e], i * STRIPE + 4 * tid + e)) { kmin = min(kmin, key_of(v[e])); kmax = max(kmax, key_of(v[e])); }
-            });
+            pass([&](float v, uint32_t idx) { if (member(v, idx)) { kmin = min(kmin, key_of(v)); kmax = max(kmax, key_of(v)); } });
             for (int o = 32; o > 0; o >>= 1) { kmin = min(kmin, __shfl_xor(kmin, o)); kmax = max(kmax, __shfl_xor(kmax, o)); }
             if (lane == 0) { atomicMin(&s.kmin, kmin); atomicMax(&s.kmax, kmax); }
             __syncthreads();
@@ -296,156 +343,205 @@ __global__ __launch_bounds__(THREADS) void k_sample_tokens(SampleArgs a)
             if (lo >= hi) break;
             const uint32_t width = 32 - __clz(hi - lo), shift = width > 11 ? width - 11 : 0;
             clear_buckets();
-            all([&](uint32_t i, const float *v, uint32_t ok) {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e++)
-                    if (((ok >> e) & 1) && member(v[e], i * STRIPE + 4 * tid + e))
-                        atomicAdd((unsigned long long *)&s.mass[(hi - key_of(v[e])) >> shift], (unsigned long long)(uint64_t)value(v[e]));
+            pass([&](float v, uint32_t idx) {
+                if (member(v, idx)) atomicAdd((unsigned long long *)&s.mass[(hi - key_of(v)) >> shift], (unsigned long long)(uint64_t)value(v));
             });
             __syncthreads();
-            find_bucket(s, tid, lane, wave, [&](uint64_t f, uint64_t) { return reached(front + f, total); });
-            if (!s.found) return;                                // (cannot be: the bucket's members sum to what the level before saw)
+            find_bucket(s, tid, lane, wave, [&](uint64_t f, uint64_t) { return reached(front + f); });
+            if (!s.found) return true;                           // (cannot be: the bucket's members sum to what the level before saw)
             front += s.before;
             const uint32_t top = hi - (s.bucket << shift);
             lo = max(lo, shift ? top - ((1u << shift) - 1) : top);
             hi = top;
         }
-        // more equal logits than the list holds: how many of them stay (each adds w), and the index of the last of those
+        // more equal logits than can be sorted: how many of them stay (each adds w), and the index of the last of those
         const uint32_t old_lim = hi == thr ? lim : 0xffffffffu;
         thr = hi;
         const uint64_t w = (uint64_t)value(value_of((uint64_t)thr << 32));
         uint64_t stay = 0, step = (uint64_t)1 << 18;             // the largest number that does not reach it, plus one
-        for (; step; step >>= 1) if (!reached(front + (stay + step) * w, total)) stay += step;
+        for (; step; step >>= 1) if (!reached(front + (stay + step) * w)) stay += step;
         stay++;
         __syncthreads();
-        all([&](uint32_t i, const float *v, uint32_t ok) {
-            uint32_t n = 0;
-#pragma unroll
-            for (uint32_t e = 0; e < 4; e++) n += ((ok >> e) & 1) && key_of(v[e]) == thr && i * STRIPE + 4 * tid + e <= old_lim;
-            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
-            if (lane == 0) s.part[i * WAVES + wave] = n;
-        });
+        s.part[tid] = 0;
         __syncthreads();
-        const uint64_t n = tid < stripes * WAVES ? s.part[tid] : 0, incl = block_scan(n, s, lane, wave);
-        if (tid == 0) s.found = 0xffffffffu;
+        pass([&](float v, uint32_t idx) { if (key_of(v) == thr && idx <= old_lim) atomicAdd((unsigned long long *)&s.part[idx >> 8], 1ull); });
+        __syncthreads();
+        uint64_t sum;
+        const uint64_t n = s.part[tid], incl = block_scan(n, s, lane, wave, sum);
+        if (tid == 0) { s.found = 0xffffffffu; s.lim = old_lim; }
         __syncthreads();
         if (incl >= stay && incl - n < stay) { s.found = tid; s.before = incl - n; }
         __syncthreads();
         const uint32_t at = s.found;
-        if (at != 0xffffffffu && wave == 0) {                   // the wave's 256 logits again, in order
+        if (at != 0xffffffffu && wave == 0) {                   // those 256 logits again, in order
             float v[4];
-            uint32_t ok = fetch(at / WAVES, (at % WAVES) * 64 + lane, v), mine = 0;
-            const uint32_t idx = at / WAVES * STRIPE + 4 * ((at % WAVES) * 64 + lane);
+            const uint32_t i = at / WAVES, t = (at % WAVES) * 64 + lane, idx = at * 256 + 4 * lane;
+            uint32_t ok = unpack(i, t, load(i, t), load_bits(i, t), v), mine = 0;
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) { if (key_of(v[e]) != thr || idx + e > old_lim) ok &= ~(1u << e); mine += (ok >> e) & 1; }
-            const uint32_t rank = wave_scan(mine, lane) - mine, want = (uint32_t)(stay - s.before);
+            for (uint32_t e = 0; e < 4; e++) { if (!(clean(v[e]) >= LOWEST) || key_of(clean(v[e])) != thr || idx + e > old_lim) ok &= ~(1u << e); mine += (ok >> e) & 1; }
+            const uint32_t rank = (uint32_t)wave_scan(mine) - mine, want = (uint32_t)(stay - s.before);
             if (rank < want && rank + mine >= want) {
                 uint32_t left = want - rank;
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) if (((ok >> e) & 1) && --left == 0) s.bucket = idx + e;
+                for (uint32_t e = 0; e < 4; e++) if (((ok >> e) & 1) && --left == 0) s.lim = min(old_lim, idx + e);
             }
         }
         __syncthreads();
-        lim = at != 0xffffffffu ? min(old_lim, s.bucket) : old_lim;
+        lim = s.lim;
         __syncthreads();
+        return true;
     };
-    // (a prefix of mass f is long enough; an empty one never is)
+    auto row_all = [&](auto f) {
+        const bool with_z = !have_z;
+        have_z = true;
+        row_from(LOWEST, f, [&](const float *v, uint32_t) { if (with_z) add_z(v); });
+    };
+
+    const bool has_k = top_k > 0 && (uint32_t)top_k < V, has_p = top_p < 1.f;
+    const uint64_t k = (uint64_t)top_k;
     const double p = (double)fmaxf(top_p, 0.f);
-    auto enough = [&](uint64_t f, uint64_t total) { return f > 0 && (double)f >= p * (double)total; };
-    uint32_t listed = 0;                                         // > 0: the kept tokens, and no others, are the first `listed` of the sorted list
-    if (top_k > 0 && (uint32_t)top_k < V) {
-        const uint64_t k = (uint64_t)top_k;
-        // k of the threads' largest logits are at least as large as what bucket B holds: so are the k largest of the row
-        uint32_t n = LIST + 1;
-        if (k <= THREADS / 2) {
-            clear_buckets();
-            if (own_mz > NINF) atomicAdd((unsigned long long *)&s.mass[bucket0(own_mz)], 1ull);
+    double own_mass = 0.0;                                       // (whole numbers below 2^53: exact)
+    uint64_t total = 0;                                          // the weight that a nucleus is a part of
+    if ((has_k && k <= THREADS / 2) || (has_p && !has_k)) {
+        // the smallest of the `want` largest of the threads' maxima: at least `want` tokens reach it
+        const uint64_t want = has_k ? k : 3 * THREADS / 4;
+        clear_buckets();
+        if (own > NINF) atomicAdd((unsigned long long *)&s.mass[bucket0(own)], 1ull);
+        if (tid == 0) s.kmin = 0xffffffffu;
+        __syncthreads();
+        find_bucket(s, tid, lane, wave, [&](uint64_t f, uint64_t) { return f >= want; });
+        const bool enough_of_them = s.found != 0;
+        float from = LOWEST;
+        if (enough_of_them) {
+            if (own > NINF && bucket0(own) <= s.bucket) atomicMin(&s.kmin, key_of(own));
             __syncthreads();
-            find_bucket(s, tid, lane, wave, [&](uint64_t f, uint64_t) { return f >= k; });
-            const uint32_t B = s.found ? s.bucket : BUCKETS - 1;
-            n = collect([&](float v, uint32_t) { return bucket0(v) <= B; });
+            from = value_of((uint64_t)s.kmin << 32);
         }
-        if (n <= LIST) {
-            sort_list(s, n, tid);
-            listed = min(n, (uint32_t)k);
-        } else {
-            shorten(one, [&](uint64_t f, uint64_t) { return f >= k; });
+        have_z = true;
+        __syncthreads();
+        row_from(from, [&](float v, uint32_t idx) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LIST) s.list[at] = ((uint64_t)key_of(v) << 32) | (uint32_t)~idx; },
+                 [&](const float *v, uint32_t ok) {
+                     add_z(v);
+                     if (!has_k) {
+#pragma unroll
+                         for (int e = 0; e < 4; e++) if (!BITS || ((ok >> e) & 1)) own_mass += weigh(v[e]);
+                     }
+                 });
+        __syncthreads();
+        listed = s.n <= LIST ? s.n : 0;
+        if (!has_k) { block_scan((uint64_t)own_mass, s, lane, wave, total); }
+        __syncthreads();
+    }
+    if (has_k) {
+        auto reached = [&](uint64_t f) { return f >= k; };
+        if (!listed) shorten(row_all, one, reached);
+        else if (listed <= 64) {
+            if (listed >= k) {                                   // (fewer: the list is everything that may be drawn)
+                if (tid < listed) s.order[tid] = s.list[tid];
+                __syncthreads();
+                border(listed, 0, one, reached);
+            }
+        } else shorten(list_pass, one, reached);
+    }
+    if (has_p) {
+        // (a prefix of mass f is long enough; an empty one never is)
+        auto reached = [&](uint64_t f) { return f > 0 && (double)f >= p * (double)total; };
+        if (has_k) {
+            // the weight of the k largest
+            own_mass = 0.0;
+            auto add = [&](float v, uint32_t idx) { if (kept(v, idx)) own_mass += weigh(v); };
+            if (listed) list_pass(add);
+            else row_all(add);
+            block_scan((uint64_t)own_mass, s, lane, wave, total);
+        }
+        bool done = false;
+        if (listed > 64) done = shorten(list_pass, weigh, reached);
+        else if (listed) {
+            // (few: one wave sorts them all; those that top-k left out become NaN, weigh nothing and sort behind)
+            own_mass = 0.0;
+            list_pass([&](float v, uint32_t idx) { if (kept(v, idx)) own_mass += weigh(v); });
+            uint64_t there;
+            block_scan((uint64_t)own_mass, s, lane, wave, there);
+            done = reached(there);
+            if (done) {
+                if (tid < listed) s.order[tid] = kept(value_of(s.list[tid]), ~(uint32_t)s.list[tid]) ? s.list[tid] : 0;
+                __syncthreads();
+                border(listed, 0, weigh, reached);
+            }
+        }
+        if (!done) {                                             // the nucleus is larger than the list
+            listed = 0;
+            shorten(row_all, weigh, reached);
         }
     }
-    if (top_p < 1.f) {
-        if (listed) {
-            run_list(listed, weigh);
-            const uint64_t total = s.run[listed - 1];
-            listed = first_reached(listed, [&](uint64_t f) { return enough(f, total); });
-        } else {
-            shorten(weigh, enough);
-        }
-    }
-    // a draw's place in the running weights: floor(u * total)
-    auto target_of = [&](uint32_t d, uint64_t total) {
+    // The weights of what is left, summed for every 256 tokens (a logit below `reach` has none: less than min_p of the largest weight, or 2^-45)
+    const double floor_w = min_p > 0.f ? (double)min_p * 17592186044416.0 : 0.0;
+    const float reach = mz - temperature * fminf(31.5f, min_p > 0.f ? 1e-3f - 0.69314718f * __builtin_amdgcn_logf(min_p) : 31.5f) * 1.00001f;
+    const float low = fmaxf(reach, LOWEST);
+    auto final_weight = [&](float v, uint32_t idx) -> uint64_t {
+        if (!(v >= low) || !kept(v, idx)) return 0;
+        const double w = weigh(v);
+        return w >= floor_w ? (uint64_t)w : 0;
+    };
+    const uint32_t parts = stripes * WAVES;
+    __syncthreads();
+    s.part[tid] = 0;
+    __syncthreads();
+    if (listed) list_pass([&](float v, uint32_t idx) { const uint64_t w = final_weight(v, idx); if (w) atomicAdd((unsigned long long *)&s.part[idx >> 8], (unsigned long long)w); });
+    else
+        row_pass([&](uint32_t at, float *v, uint32_t ok) {
+            uint64_t w = 0;
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) { v[e] = clean(v[e]); any |= v[e] >= low; }
+            if (!have_z) add_z(v);
+            if (any) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) if (!BITS || ((ok >> e) & 1)) w += final_weight(v[e], at + e);
+            }
+            if (__any(w != 0)) {
+                const uint64_t sum = wave_scan(w);
+                if (lane == 63) s.part[at >> 8] = sum;
+            }
+        });
+    __syncthreads();
+    uint64_t left;
+    const uint64_t incl = block_scan(tid < parts ? s.part[tid] : 0, s, lane, wave, left);
+    s.part[tid] = incl;
+    // ... and the sum of exponentials
+    for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o);
+    if (lane == 0) s.wavef[wave] = z;
+    __syncthreads();
+    double lse = 0.0;
+    for (int w = 0; w < WAVES; w++) lse += (double)s.wavef[w];
+    lse = (double)mx + log(lse);
+    for (uint32_t d = wave; d < a.draws; d += WAVES) {
+        // floor(u * left), and the first 256 tokens whose running sum passes it
         const float u = a.u[(uint64_t)row * a.draws + d];
         const double uc = u > 0.f ? fmin((double)u, 1.0 - 1.0 / 16777216) : 0.0;
         const uint64_t u63 = (uint64_t)(uc * 9223372036854775808.0);
-        return (__umul64hi(u63, total) << 1) | ((u63 * total) >> 63);
-    };
-    auto put = [&](uint32_t d, uint32_t idx, float v) {
-        a.tokens[(uint64_t)row * a.draws + d] = idx;
-        a.logprobs[(uint64_t)row * a.draws + d] = (float)((double)v - lse);
-    };
-    auto floored = [&](float v) { const double w = weigh(v); return w >= floor_w ? w : 0.0; };
-    if (listed) {
-        // into the order of the vocabulary: (~index << 32 | key) falls as the index rises
-        __syncthreads();
-        for (uint32_t i = tid; i < listed; i += THREADS) s.list[i] = (s.list[i] << 32) | (s.list[i] >> 32);
-        sort_list(s, listed, tid);
-        for (uint32_t i = tid; i < listed; i += THREADS) s.list[i] = (s.list[i] << 32) | (s.list[i] >> 32);
-        __syncthreads();
-        run_list(listed, floored);
-        const uint64_t total = s.run[listed - 1];
-        for (uint32_t d = tid; d < a.draws; d += THREADS) {
-            const uint64_t target = target_of(d, total);
-            uint32_t lo = 0, hi = listed - 1;
-            while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (s.run[mid] > target) hi = mid; else lo = mid + 1; }
-            put(d, ~(uint32_t)s.list[lo], value_of(s.list[lo]));
-        }
-        return;
-    }
-    // the weights of what is left, summed for every 256 tokens (a logit below `reach` has none: less than min_p of the largest weight, or 2^-45)
-    const float reach = mz - temperature * fminf(31.5f, floor_w > 0.0 ? 1e-3f - 0.69314718f * __builtin_amdgcn_logf(fminf(min_p_, 1.f)) : 31.5f) * 1.00001f;
-    auto final_weight = [&](float v, uint32_t idx, uint32_t ok) -> uint64_t { return ok && !(v < reach) && kept(v, idx) ? (uint64_t)floored(v) : 0; };
-    __syncthreads();
-    all([&](uint32_t i, const float *v, uint32_t ok) {
-        uint64_t w = 0;
-#pragma unroll
-        for (uint32_t e = 0; e < 4; e++) w += final_weight(v[e], i * STRIPE + 4 * tid + e, (ok >> e) & 1);
-        if (__any(w != 0))
-            for (int o = 32; o > 0; o >>= 1) w += __shfl_xor(w, o);
-        if (lane == 0) s.part[i * WAVES + wave] = w;
-    });
-    __syncthreads();
-    const uint32_t parts = stripes * WAVES;
-    const uint64_t incl = block_scan(tid < parts ? s.part[tid] : 0, s, lane, wave);
-    if (tid < parts) s.part[tid] = incl;
-    __syncthreads();
-    const uint64_t total = s.part[parts - 1];
-    for (uint32_t d = wave; d < a.draws; d += WAVES) {
-        const uint64_t target = target_of(d, total);
-        uint32_t lo = 0, hi = parts - 1;                         // the first part whose running sum passes the target
+        const uint64_t target = (__umul64hi(u63, left) << 1) | ((u63 * left) >> 63);
+        uint32_t lo = 0, hi = parts - 1;
         while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (s.part[mid] > target) hi = mid; else lo = mid + 1; }
         const uint64_t rest = target - (lo ? s.part[lo - 1] : 0);
         float v[4];
-        const uint32_t t = (lo % WAVES) * 64 + lane, ok = fetch(lo / WAVES, t, v), idx = lo / WAVES * STRIPE + 4 * t;
-        uint64_t w[4], mine = 0;
+        uint64_t w[4];
+        const uint32_t i = lo / WAVES, t = (lo % WAVES) * 64 + lane, idx = lo * 256 + 4 * lane;
+        const uint32_t ok = unpack(i, t, load(i, t), load_bits(i, t), v);
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++) { w[e] = final_weight(v[e], idx + e, (ok >> e) & 1); mine += w[e]; }
-        const uint64_t sum = wave_scan(mine, lane);
+        for (uint32_t e = 0; e < 4; e++) { v[e] = clean(v[e]); w[e] = !BITS || ((ok >> e) & 1) ? final_weight(v[e], idx + e) : 0; }
+        const uint64_t mine = w[0] + w[1] + w[2] + w[3], sum = wave_scan(mine);
         if (sum > rest && sum - mine <= rest) {
             uint64_t run = sum - mine;
             bool done = false;
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) {
                 run += w[e];
-                if (!done && run > rest) { done = true; put(d, idx + e, v[e]); }
+                if (!done && run > rest) {
+                    done = true;
+                    a.tokens[(uint64_t)row * a.draws + d] = idx + e;
+                    a.logprobs[(uint64_t)row * a.draws + d] = (float)((double)v[e] - lse);
+                }
             }
         }
     }
@@ -457,7 +553,8 @@ static int sample_tokens(void *stream, const SampleArgs &a)
     if (!a.rows || !a.draws) return FMI_OK;
     if (!a.vocab || a.vocab > MAX_VOCAB) { fmi_set_error("sealnn_sample_tokens: a vocabulary of %u (1 .. %u)", a.vocab, (unsigned)MAX_VOCAB); return FMI_ERR_UNSUPPORTED; }
     if (!a.logits || !a.u || !a.tokens || !a.logprobs || ((uintptr_t)a.logits & (sizeof(T) - 1))) { fmi_set_error("sealnn_sample_tokens: null or misaligned argument"); return FMI_ERR_ARG; }
-    hipLaunchKernelGGL(k_sample_tokens<T>, dim3(a.rows), dim3(THREADS), 0, (hipStream_t)stream, a);
+    if (a.bits) hipLaunchKernelGGL((k_sample_tokens<T, true>), dim3(a.rows), dim3(THREADS), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((k_sample_tokens<T, false>), dim3(a.rows), dim3(THREADS), 0, (hipStream_t)stream, a);
     NNCHK();
     return FMI_OK;
 }
