@@ -219,24 +219,22 @@ def uint64s(*values):
     return (_u64 * len(values))(*values)
 
 
-class launch_on:
-    """``with launch_on(tensor) as stream``: the current stream of the tensor's device (its address), that device current while the call is made"""
-    __slots__ = ("index", "old")
-
-    def __init__(self, tensor):
-        self.index = tensor.device.index
-
-    def __enter__(self):
-        import torch
-        self.old = torch.cuda.current_device()
-        if self.old != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.old != self.index:
-            import torch
-            torch.cuda.set_device(self.old)
+def launch(fn, index: int, *args) -> None:
+    """``check(fn(stream, *args))`` with the current stream of device ``index``, that device current while the call is made (a decode step is many small calls: what
+    this costs is a part of their time)"""
+    import torch
+    C = torch._C
+    old = C._cuda_getDevice()
+    if old == index:
+        rc = fn(C._cuda_getCurrentRawStream(index), *args)
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = fn(C._cuda_getCurrentRawStream(index), *args)
+        finally:
+            torch.cuda.set_device(old)
+    if rc:
+        check(rc)
 
 
 def check(rc: int) -> None:

@@ -8,7 +8,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, launch_on, lib, uint64s
+from ._lib import launch, lib, uint64s
 
 TILE = 64                                  # tokens of a tile of the layout
 WAVES_WANTED = 4096                        # waves that keep the memory of 256 CUs busy
@@ -20,24 +20,22 @@ class KV8Cache:
     ``KV8Cache.empty`` makes the buffers."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        self._check(k, v, k_scale, v_scale)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.slots, self.heads, self.tokens, self.head_dim = k.shape
-        self.block = self.tokens // k_scale.shape[2]
-
-    @staticmethod
-    def _check(k, v, k_scale, v_scale):
-        if k.dim() != 4 or k.shape[3] not in (64, 128) or k.shape[2] % TILE or not k.shape[2]:
-            raise ValueError(f"KV8Cache: k is [slots, heads, T, head_dim] with T a multiple of {TILE} and head_dim 64 or 128, got {tuple(k.shape)}")
-        S, H, T, D = k.shape
+        shape, blocks = k.shape, k_scale.shape
+        if len(shape) != 4 or shape[3] not in (64, 128) or shape[2] % TILE or not shape[2]:
+            raise ValueError(f"KV8Cache: k is [slots, heads, T, head_dim] with T a multiple of {TILE} and head_dim 64 or 128, got {tuple(shape)}")
+        S, H, T, D = shape
         if v.shape != (S, H, T // TILE, D, TILE):
             raise ValueError(f"KV8Cache: v is {(S, H, T // TILE, D, TILE)}, got {tuple(v.shape)}")
-        if k_scale.dim() != 3 or k_scale.shape[:2] != (S, H) or k_scale.shape != v_scale.shape or k_scale.shape[2] not in (T // 16, T // 32, T // 64):
-            raise ValueError(f"KV8Cache: the scales are [{S}, {H}, T / block] with a block of 16, 32 or 64 tokens, got {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
+        if len(blocks) != 3 or blocks[0] != S or blocks[1] != H or blocks != v_scale.shape or blocks[2] not in (T // 16, T // 32, T // 64):
+            raise ValueError(f"KV8Cache: the scales are [{S}, {H}, T / block] with a block of 16, 32 or 64 tokens, got {tuple(blocks)} and {tuple(v_scale.shape)}")
         if k.dtype != torch.uint8 or v.dtype != torch.uint8 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
             raise ValueError("KV8Cache: codes are uint8 and scales fp32")
-        if any(t.device != k.device or not t.is_contiguous() for t in (k, v, k_scale, v_scale)):
+        dev = k.device
+        if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
+                and dev == v.device == k_scale.device == v_scale.device):
             raise ValueError("KV8Cache: the four tensors must be contiguous and on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.slots, self.heads, self.tokens, self.head_dim, self.block, self.device = S, H, T, D, T // blocks[2], dev
 
     @classmethod
     def empty(cls, slots: int, heads: int, tokens: int, head_dim: int = 64, block: int = 16, device="cuda") -> "KV8Cache":
@@ -49,69 +47,66 @@ class KV8Cache:
                    torch.zeros(slots, heads, T // TILE, head_dim, TILE, dtype=torch.uint8, device=device),
                    torch.full((slots, heads, T // block), 2.0 ** -64, device=device), torch.full((slots, heads, T // block), 2.0 ** -64, device=device))
 
-    def _on_gpu(self):
+    def _lengths(self, t: torch.Tensor, name: str):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != self.slots or t.device != self.device or not t.is_contiguous():
+            raise ValueError(f"KV8Cache: {name} is int32 [{self.slots}], contiguous, on {self.device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.data_ptr()
+
+    def _on_gpu(self) -> int:
         if not self.k.is_cuda:
             raise RuntimeError("KV8Cache: the cache must live on the GPU (seal_amd has no CPU path)")
-
-    def _lengths(self, t: torch.Tensor, name: str):
-        if t.dtype != torch.int32 or t.shape != (self.slots,) or t.device != self.k.device or not t.is_contiguous():
-            raise ValueError(f"KV8Cache: {name} is int32 [{self.slots}], contiguous, on {self.k.device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
-        return t.data_ptr()
+        return self.k.get_device()
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
         """Write ``k_new`` / ``v_new`` [slots, n, heads, head_dim] (fp32 or bf16; any strides, dims contiguous) at positions ``lengths[slot]`` .. of every
         slot: all n tokens, or the first ``counts[slot]`` of them.  What would lie behind the cache's end is dropped.  ``lengths`` (int32 [slots], on the
         device) is left as it is: the caller counts."""
-        n = k_new.shape[1] if k_new.dim() == 4 else -1
-        for t in (k_new, v_new):
-            if t.shape != (self.slots, n, self.heads, self.head_dim) or t.dtype != k_new.dtype or t.device != self.k.device:
-                raise ValueError(f"KV8Cache.append: keys and values are [{self.slots}, n, {self.heads}, {self.head_dim}] of one type on {self.k.device}, "
-                                 f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-            if t.stride(3) != 1:
-                raise ValueError("KV8Cache.append: the dims of a head must be contiguous")
-        if k_new.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"KV8Cache.append: fp32 or bf16, got {k_new.dtype}")
+        shape, dt = k_new.shape, k_new.dtype
+        if (len(shape) != 4 or shape[0] != self.slots or shape[2] != self.heads or shape[3] != self.head_dim or v_new.shape != shape or v_new.dtype != dt
+                or k_new.device != self.device or v_new.device != self.device):
+            raise ValueError(f"KV8Cache.append: keys and values are [{self.slots}, n, {self.heads}, {self.head_dim}] of one type on {self.device}, "
+                             f"got {dt} {tuple(shape)} on {k_new.device} and {v_new.dtype} {tuple(v_new.shape)} on {v_new.device}")
+        if dt != torch.float32 and dt != torch.bfloat16:
+            raise ValueError(f"KV8Cache.append: fp32 or bf16, got {dt}")
+        ks, vs = k_new.stride(), v_new.stride()
+        if ks[3] != 1 or vs[3] != 1:
+            raise ValueError("KV8Cache.append: the dims of a head must be contiguous")
         lengths_ptr, counts_ptr = self._lengths(lengths, "lengths"), None if counts is None else self._lengths(counts, "counts")
-        self._on_gpu()
-        fn = lib().sealnn_kv8_append if k_new.dtype == torch.float32 else lib().sealnn_kv8_append_bf16
-        strides = uint64s(*k_new.stride()[:3], *v_new.stride()[:3])
-        with launch_on(self.k) as stream:
-            check(fn(stream, k_new.data_ptr(), v_new.data_ptr(), strides, n, lengths_ptr, counts_ptr, self.k.data_ptr(), self.v.data_ptr(),
-                     self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.slots, self.heads, self.tokens, self.block, self.head_dim))
+        launch(lib().sealnn_kv8_append if dt == torch.float32 else lib().sealnn_kv8_append_bf16, self._on_gpu(), k_new.data_ptr(), v_new.data_ptr(),
+               uint64s(ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), shape[1], lengths_ptr, counts_ptr, self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+               self.v_scale.data_ptr(), self.slots, self.heads, self.tokens, self.block, self.head_dim)
 
     def attend(self, q: torch.Tensor, lengths: torch.Tensor, beams: int = 1, keep: Optional[torch.Tensor] = None,
                scale: Optional[float] = None) -> torch.Tensor:
         """softmax(scale q K^T) V: ``q`` [slots * beams, q_heads, head_dim] (fp32 or bf16; rows and heads may be strided; row r reads slot r // beams, head h
         reads cached head h // (q_heads / heads)) over the first ``lengths[slot]`` tokens, those of them for which ``keep`` (bool or uint8 [slots, T]) is set.
         ``scale`` defaults to head_dim ** -0.5.  A row with nothing to attend to is zeros.  Returns a new tensor shaped and typed like ``q``."""
-        D, H = self.head_dim, self.heads
-        if (q.dim() != 3 or beams < 1 or q.shape[0] != self.slots * beams or q.shape[2] != D or q.shape[1] % H or not q.shape[1]
-                or q.dtype not in (torch.float32, torch.bfloat16) or q.device != self.k.device):
-            raise ValueError(f"KV8Cache.attend: q is fp32 or bf16 [{self.slots} * beams, a multiple of {H}, {D}] on {self.k.device}, "
-                             f"got {q.dtype} {tuple(q.shape)} on {q.device}")
-        if q.stride(2) != 1:
+        D, H, shape, dt = self.head_dim, self.heads, q.shape, q.dtype
+        if (len(shape) != 3 or beams < 1 or shape[0] != self.slots * beams or shape[2] != D or shape[1] % H or not shape[1]
+                or (dt != torch.float32 and dt != torch.bfloat16) or q.device != self.device):
+            raise ValueError(f"KV8Cache.attend: q is fp32 or bf16 [{self.slots} * beams, a multiple of {H}, {D}] on {self.device}, "
+                             f"got {dt} {tuple(shape)} on {q.device}")
+        row_stride, head_stride, stride = q.stride()
+        if stride != 1:
             raise ValueError("KV8Cache.attend: the dims of a head must be contiguous")
-        share = q.shape[1] // H
+        share = shape[1] // H
         keep_ptr, keep_stride = None, 0
         if keep is not None:
-            if keep.shape != (self.slots, self.tokens) or keep.dtype not in (torch.bool, torch.uint8) or keep.device != self.k.device:
-                raise ValueError(f"KV8Cache.attend: keep is bool or uint8 [{self.slots}, {self.tokens}] on {self.k.device}, got {keep.dtype} {tuple(keep.shape)}")
+            if keep.shape != (self.slots, self.tokens) or keep.dtype not in (torch.bool, torch.uint8) or keep.device != self.device:
+                raise ValueError(f"KV8Cache.attend: keep is bool or uint8 [{self.slots}, {self.tokens}] on {self.device}, got {keep.dtype} {tuple(keep.shape)}")
             keep = keep.contiguous()
             keep_ptr, keep_stride = keep.data_ptr(), self.tokens
-        lengths_ptr = self._lengths(lengths, "lengths")
-        self._on_gpu()
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lengths_ptr, index = self._lengths(lengths, "lengths"), self._on_gpu()
+        out = q.new_empty(shape)
         items = self.slots * H * ((beams * share + 15) // 16)
         splits = max(1, min(self.tokens // TILE // 4, WAVES_WANTED // 4 // max(items, 1)))
-        work, work_bytes = None, 0
+        work, work_floats = None, 0
         if splits > 1:
-            work = torch.empty(items * splits * 16 * (D + 4), dtype=torch.float32, device=q.device)
-            work_bytes = work.numel() * 4
-        fn = lib().sealnn_kv8_attend if q.dtype == torch.float32 else lib().sealnn_kv8_attend_bf16
-        with launch_on(q) as stream:
-            check(fn(stream, q.data_ptr(), q.stride(0), q.stride(1), self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                     lengths_ptr, keep_ptr, keep_stride, self.slots, beams, H, share, self.tokens, self.block, D,
-                     D ** -0.5 if scale is None else float(scale), splits, None if work is None else work.data_ptr(), work_bytes, out.data_ptr()))
+            work_floats = items * splits * 16 * (D + 4)
+            work = torch.empty(work_floats, dtype=torch.float32, device=self.device)
+        launch(lib().sealnn_kv8_attend if dt == torch.float32 else lib().sealnn_kv8_attend_bf16, index, q.data_ptr(), row_stride, head_stride, self.k.data_ptr(),
+               self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), lengths_ptr, keep_ptr, keep_stride, self.slots, beams, H, share, self.tokens,
+               self.block, D, D ** -0.5 if scale is None else scale, splits, None if work is None else work.data_ptr(), work_floats * 4, out.data_ptr())
         return out
 
     def values(self):

@@ -7,20 +7,18 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from ._lib import check, launch_on, lib
+from ._lib import launch, lib
 
 MAX_VOCAB = 1 << 18
 Setting = Union[float, int, torch.Tensor]
 
 
-def _setting(value: Setting, name: str, rows: int, dtype: torch.dtype, like: torch.Tensor):
-    """(number, address of a per-row tensor or None) of a sampling parameter"""
-    if isinstance(value, torch.Tensor):
-        if value.dtype != dtype or value.shape != (rows,) or value.device != like.device or not value.is_contiguous():
-            raise ValueError(f"sample_tokens: {name} as a tensor is {dtype}, one value for each of the {rows} rows, contiguous, on {like.device} "
-                             f"(got {value.dtype}, {tuple(value.shape)}, {value.device})")
-        return 0, value.data_ptr()
-    return value, None
+def _per_row(value: torch.Tensor, name: str, rows: int, dtype: torch.dtype, device) -> int:
+    """the address of a sampling parameter that every row has its own of"""
+    if value.dtype != dtype or value.shape != (rows,) or value.device != device or not value.is_contiguous():
+        raise ValueError(f"sample_tokens: {name} as a tensor is {dtype}, one value for each of the {rows} rows, contiguous, on {device} "
+                         f"(got {value.dtype}, {tuple(value.shape)}, {value.device})")
+    return value.data_ptr()
 
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0, top_p: Setting = 1.0,
@@ -36,44 +34,57 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
 
     A row of which no token may be drawn gives token -1 and log-probability -inf.  ``logprobs`` are those of the model: ``logit - logsumexp`` of the whole
     row, without temperature, constraint or filters (what the decode loop carries, as the reference's beam scores carry unconstrained ones)."""
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"sample_tokens: logits are fp32 or bf16 [rows, vocab], got {logits.dtype} {tuple(logits.shape)}")
-    rows, vocab = logits.shape
+    dt, shape, dev, u_shape = logits.dtype, logits.shape, logits.device, u.shape
+    if len(shape) != 2 or (dt != torch.float32 and dt != torch.bfloat16):
+        raise ValueError(f"sample_tokens: logits are fp32 or bf16 [rows, vocab], got {dt} {tuple(shape)}")
+    rows, vocab = shape
     if not 0 < vocab <= MAX_VOCAB:
         raise ValueError(f"sample_tokens: a vocabulary of 1 .. {MAX_VOCAB} tokens, got {vocab}")
-    if vocab > 1 and logits.stride(1) != 1:
+    row_stride, stride = logits.stride()
+    if stride != 1 and vocab > 1:
         raise ValueError("sample_tokens: the logits of a row must be contiguous")
-    if rows > 1 and logits.stride(0) < vocab:
+    if row_stride < vocab and rows > 1:
         raise ValueError("sample_tokens: the rows of the logits overlap")
-    if u.dtype != torch.float32 or u.dim() not in (1, 2) or u.shape[0] != rows or u.device != logits.device:
-        raise ValueError(f"sample_tokens: u is fp32 [rows] or [rows, draws] on {logits.device}, got {u.dtype} {tuple(u.shape)} on {u.device}")
+    if u.dtype != torch.float32 or not 0 < len(u_shape) < 3 or u_shape[0] != rows or u.device != dev:
+        raise ValueError(f"sample_tokens: u is fp32 [rows] or [rows, draws] on {dev}, got {u.dtype} {tuple(u_shape)} on {u.device}")
     u = u.contiguous()
-    if not isinstance(temperature, torch.Tensor) and not 0 <= temperature < float("inf"):
+    t = k = p = m = 0
+    t_v = k_v = p_v = m_v = None
+    if isinstance(temperature, torch.Tensor):
+        t_v = _per_row(temperature, "temperature", rows, torch.float32, dev)
+    elif 0 <= temperature < float("inf"):
+        t = temperature
+    else:
         raise ValueError(f"sample_tokens: temperature = {temperature}")
-    if not isinstance(top_k, torch.Tensor) and (top_k < 0 or top_k != int(top_k)):
+    if isinstance(top_k, torch.Tensor):
+        k_v = _per_row(top_k, "top_k", rows, torch.int32, dev)
+    elif top_k >= 0 and top_k == int(top_k):
+        k = min(int(top_k), MAX_VOCAB)
+    else:
         raise ValueError(f"sample_tokens: top_k = {top_k}")
-    if not isinstance(top_p, torch.Tensor) and not 0 <= top_p <= 1:
+    if isinstance(top_p, torch.Tensor):
+        p_v = _per_row(top_p, "top_p", rows, torch.float32, dev)
+    elif 0 <= top_p <= 1:
+        p = top_p
+    else:
         raise ValueError(f"sample_tokens: top_p = {top_p}")
-    if not isinstance(min_p, torch.Tensor) and not 0 <= min_p <= 1:
+    if isinstance(min_p, torch.Tensor):
+        m_v = _per_row(min_p, "min_p", rows, torch.float32, dev)
+    elif 0 <= min_p <= 1:
+        m = min_p
+    else:
         raise ValueError(f"sample_tokens: min_p = {min_p}")
-    t, t_v = _setting(temperature, "temperature", rows, torch.float32, logits)
-    k, k_v = _setting(top_k, "top_k", rows, torch.int32, logits)
-    p, p_v = _setting(top_p, "top_p", rows, torch.float32, logits)
-    m, m_v = _setting(min_p, "min_p", rows, torch.float32, logits)
     bits, bits_stride = None, 0
     if allowed_bits is not None:
-        b = allowed_bits
-        if (b.dtype != torch.int32 or b.dim() != 2 or b.shape[0] != rows or b.shape[1] < (vocab + 31) // 32 or b.device != logits.device
-                or (b.shape[1] > 1 and b.stride(1) != 1)):
-            raise ValueError(f"sample_tokens: allowed_bits is int32 [rows, >= {(vocab + 31) // 32}] with contiguous rows on {logits.device}, "
-                             f"got {b.dtype} {tuple(b.shape)} on {b.device}")
-        bits, bits_stride = b.data_ptr(), b.stride(0)
+        b_shape = allowed_bits.shape
+        if (allowed_bits.dtype != torch.int32 or len(b_shape) != 2 or b_shape[0] != rows or b_shape[1] < (vocab + 31) // 32 or allowed_bits.device != dev
+                or (allowed_bits.stride(1) != 1 and b_shape[1] > 1)):
+            raise ValueError(f"sample_tokens: allowed_bits is int32 [rows, >= {(vocab + 31) // 32}] with contiguous rows on {dev}, "
+                             f"got {allowed_bits.dtype} {tuple(b_shape)} on {allowed_bits.device}")
+        bits, bits_stride = allowed_bits.data_ptr(), allowed_bits.stride(0)
     if not logits.is_cuda:
         raise RuntimeError("sample_tokens: the logits must live on the GPU (seal_amd has no CPU path)")
-    tokens = torch.empty(u.shape, dtype=torch.int64, device=u.device)
-    logprobs = torch.empty_like(u)
-    fn = lib().sealnn_sample_tokens if logits.dtype == torch.float32 else lib().sealnn_sample_tokens_bf16
-    with launch_on(logits) as stream:
-        check(fn(stream, logits.data_ptr(), logits.stride(0), rows, vocab, u.data_ptr(), u.shape[1] if u.dim() == 2 else 1, bits, bits_stride,
-                 t, min(int(k), MAX_VOCAB), p, m, t_v, k_v, p_v, m_v, tokens.data_ptr(), logprobs.data_ptr()))
+    tokens, logprobs = u.new_empty(u_shape, dtype=torch.int64), u.new_empty(u_shape)
+    launch(lib().sealnn_sample_tokens if dt == torch.float32 else lib().sealnn_sample_tokens_bf16, logits.get_device(), logits.data_ptr(), row_stride, rows, vocab,
+           u.data_ptr(), u_shape[1] if len(u_shape) == 2 else 1, bits, bits_stride, t, k, p, m, t_v, k_v, p_v, m_v, tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs

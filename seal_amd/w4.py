@@ -7,7 +7,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, launch_on, lib
+from ._lib import launch, lib
 
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -65,17 +65,18 @@ def quantize_w4(weight: torch.Tensor, group: int = 32) -> W4Weight:
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None, gelu: bool = False) -> torch.Tensor:
     """``F.linear(x, weight, bias)`` (and its erf GELU) for ``x`` fp32 or bf16 [rows, in_features], rows may be strided; ``bias`` of x's type.  Made for 1 .. 64 rows; any
     number works.  Returns a new [rows, out_features] of x's type."""
-    if x.dim() != 2 or x.shape[1] != weight.in_features or x.dtype not in (torch.float32, torch.bfloat16) or x.device != weight.codes.device:
-        raise ValueError(f"w4_linear: x is fp32 or bf16 [rows, {weight.in_features}] on {weight.codes.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    codes, dt = weight.codes, x.dtype
+    if x.dim() != 2 or x.shape[1] != weight.in_features or (dt != torch.float32 and dt != torch.bfloat16) or x.device != codes.device:
+        raise ValueError(f"w4_linear: x is fp32 or bf16 [rows, {weight.in_features}] on {codes.device}, got {dt} {tuple(x.shape)} on {x.device}")
+    rows, N = x.shape[0], weight.out_features
+    row_stride, stride = x.stride()
+    if stride != 1 and weight.in_features > 1:
         raise ValueError("w4_linear: the columns of a row of x must be contiguous")
-    if bias is not None and (bias.shape != (weight.out_features,) or bias.dtype != x.dtype or bias.device != x.device or not bias.is_contiguous()):
-        raise ValueError(f"w4_linear: the bias is {x.dtype} [{weight.out_features}], contiguous, on {x.device}")
+    if bias is not None and (bias.shape != (N,) or bias.dtype != dt or bias.device != x.device or not bias.is_contiguous()):
+        raise ValueError(f"w4_linear: the bias is {dt} [{N}], contiguous, on {x.device}")
     if not x.is_cuda:
         raise RuntimeError("w4_linear: x must live on the GPU (seal_amd has no CPU path)")
-    y = torch.empty(x.shape[0], weight.out_features, dtype=x.dtype, device=x.device)
-    fn = lib().sealnn_w4_linear if x.dtype == torch.float32 else lib().sealnn_w4_linear_bf16
-    with launch_on(x) as stream:
-        check(fn(stream, x.data_ptr(), x.stride(0), weight.codes.data_ptr(), weight.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                 x.shape[0], weight.out_features, weight.in_features, weight.group, int(gelu), y.data_ptr()))
+    y = x.new_empty((rows, N))
+    launch(lib().sealnn_w4_linear if dt == torch.float32 else lib().sealnn_w4_linear_bf16, x.get_device(), x.data_ptr(), row_stride, codes.data_ptr(),
+           weight.scales.data_ptr(), None if bias is None else bias.data_ptr(), rows, N, weight.in_features, weight.group, gelu, y.data_ptr())
     return y
