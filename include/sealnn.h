@@ -168,7 +168,7 @@ int sealnn_kv8_append_bf16(void *stream, const void *k_new, const void *v_new, c
                            uint32_t block, uint32_t dh);
 /* out [slots * beams][heads * share][dh] = softmax(scale q K^T) V over the first lengths[slot] tokens of the row's slot (row / beams) whose
  * keep[slot * keep_stride + token] is not 0 (keep NULL: all); nothing left: zeros.  Query head h reads cached head h / share.  splits > 1: the tokens
- * of every slot in `splits` parts, joined by a second launch; `work` then holds slots * heads * ceil(beams * share / 16) * splits * 16 * (dh + 4) floats. */
+ * of every slot in `splits` parts, joined by a second launch; `work` then holds slots * beams * heads * share * splits * (dh + 4) floats. */
 int sealnn_kv8_attend(void *stream, const float *q, uint64_t q_row_stride, uint64_t q_head_stride, const void *k, const void *v,
                       const float *k_scale, const float *v_scale, const int32_t *lengths, const uint8_t *keep, uint64_t keep_stride,
                       uint32_t slots, uint32_t beams, uint32_t heads, uint32_t share, uint32_t T, uint32_t block, uint32_t dh, float scale,

@@ -202,8 +202,8 @@ struct AttendArgs {
     const uint8_t *keep;             // [slots][keep_stride] or null
     uint64_t keep_stride;
     void *out;
-    float *part;                     // [items][splits][16][dh + 2] when splits > 1
-    uint32_t slots, heads, share, beams, T, block, splits, qtiles;
+    float *part;                     // [slots][heads][beams * share][splits][dh + 4] when splits > 1
+    uint32_t slots, heads, share, beams, T, block, splits, qtiles, items, vec;
     float scale2;                    // scale * log2(e)
 };
 
@@ -221,67 +221,102 @@ static __device__ __forceinline__ bf16x8 bytes8(uint32_t a, uint32_t b)
     return __builtin_bit_cast(bf16x8, o);
 }
 
+// what a wave needs of a tile of 64 tokens, as it lies in memory: K's rows with scales and mask bytes, V's rows
+template <int DH> struct TileK {
+    u32x4 k[4][DH / 64];
+    float ks[4], vs[4];
+    uint32_t keep[4];
+};
+template <int DH>
+static __device__ __forceinline__ void load_k(const AttendArgs &a, const uint8_t *kb, const float *ksc, const float *vsc, const uint8_t *keep, uint32_t t, uint32_t subtiles,
+                                              uint32_t c, uint32_t g, TileK<DH> &x)
+{
+    const uint32_t base = t * 64;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (j < (int)subtiles) {                                 // (a short tile: its last sixteens are not read)
+#pragma unroll
+            for (int h = 0; h < DH / 64; h++) x.k[j][h] = *(const u32x4 *)(kb + (uint64_t)(base + 16 * j + c) * DH + 64 * h + 16 * g);
+        } else {
+#pragma unroll
+            for (int h = 0; h < DH / 64; h++) x.k[j][h] = u32x4{0, 0, 0, 0};
+        }
+        const uint32_t b = (base + 16 * j) / a.block;
+        x.ks[j] = ksc[b];
+        x.vs[j] = vsc[b];
+        x.keep[j] = keep ? *(const uint32_t *)(keep + base + 16 * j + 4 * g) : 0x01010101u;
+    }
+}
+template <int DH>
+static __device__ __forceinline__ void load_v(const uint8_t *vb, uint32_t t, uint32_t c, uint32_t g, u32x4 v[DH / 16])
+{
+#pragma unroll
+    for (int d = 0; d < DH / 16; d++) v[d] = *(const u32x4 *)(vb + (uint64_t)t * 64 * DH + (16 * d + c) * 64 + 16 * g);
+}
+
+// WAVES > 1: a workgroup per (slot, head, 16 queries, part of the tokens), its waves take the tiles in turn and are joined in LDS.  WAVES == 1 (one tile is all there is): four
+// waves of a workgroup with an item each.
 template <typename T_, int DH, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_kv8_attend(AttendArgs a)
+__global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void k_kv8_attend(AttendArgs a)
 {
     enum { HALVES = DH / 64, DT = DH / 16, NQ = QP<T_>::Q, NP = QP<T_>::P };
     const float NINF = -__builtin_huge_valf();
     __shared__ float s_m[WAVES][16], s_l[WAVES][16];
-    __shared__ f32x4 s_o[WAVES > 1 ? WAVES : 1][DT][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const uint32_t item = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    __shared__ f32x4 s_o[WAVES][WAVES > 1 ? DT : 1][64];
+    // (the wave's number as a scalar: what follows from it -- slot, lengths, scales, base addresses -- stays out of the vector registers)
+    const uint32_t lane = threadIdx.x & 63, w4 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wave = WAVES > 1 ? w4 : 0, c = lane & 15, g = lane >> 4;
+    const uint32_t id = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + w4;
+    if (id >= a.items * a.splits) return;
+    const uint32_t item = id / a.splits, split = id % a.splits;
     const uint32_t qt = item % a.qtiles, sh = item / a.qtiles, slot = sh / a.heads, head = sh % a.heads;
     const int32_t raw = a.lengths[slot];
     const uint32_t len = raw < 0 ? 0 : min((uint32_t)raw, a.T), tiles = (len + 63) / 64;
     const uint32_t t_begin = (uint32_t)((uint64_t)tiles * split / a.splits), t_end = (uint32_t)((uint64_t)tiles * (split + 1) / a.splits);
+    const uint8_t *kb = a.k + (uint64_t)sh * a.T * DH, *vb = a.v + (uint64_t)sh * a.T * DH;
+    const float *ksc = a.k_scale + (uint64_t)sh * (a.T / a.block), *vsc = a.v_scale + (uint64_t)sh * (a.T / a.block);
+    const uint8_t *keep = a.keep ? a.keep + slot * a.keep_stride : nullptr;
+    uint32_t t = t_begin + wave;
+    TileK<DH> x;
+    u32x4 v[DT];
+    if (t < t_end) { load_k<DH>(a, kb, ksc, vsc, keep, t, min(4u, (len - 64 * t + 15) / 16), c, g, x); load_v<DH>(vb, t, c, g, v); }
     const uint32_t queries = a.beams * a.share, qi = qt * 16 + c;
     const bool live = qi < queries;
     const uint64_t row = (uint64_t)slot * a.beams + (live ? qi / a.share : 0);
     const uint32_t hq = head * a.share + (live ? qi % a.share : 0);
     bf16x8 q[HALVES][2][NQ];
     {
-        const T_ *p = (const T_ *)a.q + row * a.q_row + (uint64_t)hq * a.q_head;
+        const T_ *p = (const T_ *)a.q + row * a.q_row + (uint64_t)hq * a.q_head + 16 * g;
 #pragma unroll
-        for (int h = 0; h < HALVES; h++)
+        for (int h = 0; h < HALVES; h++) {
+            float y[16];
+            if (live) load16(p + 64 * h, a.vec, y);
+#pragma unroll
+            for (int i = 0; i < 16; i++) y[i] = live ? y[i] : 0.f;
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = live ? load1(p + 64 * h + 16 * g + 8 * s + i) : 0.f;
                 Planes pl;
-                split8(x, pl);
+                split8(y + 8 * s, pl);
 #pragma unroll
                 for (int n = 0; n < NQ; n++) q[h][s][n] = pl.p[n];
             }
+        }
     }
     float m = NINF, l = 0.f;
     f32x4 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint8_t *kb = a.k + (uint64_t)sh * a.T * DH, *vb = a.v + (uint64_t)sh * a.T * DH;
-    const float *ksc = a.k_scale + (uint64_t)sh * (a.T / a.block), *vsc = a.v_scale + (uint64_t)sh * (a.T / a.block);
-    for (uint32_t t = t_begin + wave; t < t_end; t += WAVES) {
+    while (t < t_end) {
+        // the next tile's K is in flight while this one is worked on, its V while the next scores are
         const uint32_t base = t * 64;
-        u32x4 kw[4][HALVES], vw[DT];
+        TileK<DH> y;
+        t += WAVES;
+        if (WAVES > 1 && t < t_end) load_k<DH>(a, kb, ksc, vsc, keep, t, 4, c, g, y);
+        uint32_t ok = 0;                                         // bit 4 j + r: token 16 j + 4 g + r counts
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int h = 0; h < HALVES; h++) kw[j][h] = *(const u32x4 *)(kb + (uint64_t)(base + 16 * j + c) * DH + 64 * h + 16 * g);
-#pragma unroll
-        for (int d = 0; d < DT; d++) vw[d] = *(const u32x4 *)(vb + (uint64_t)base * DH + (16 * d + c) * 64 + 16 * g);
-        float ks[4], vs[4];
-        uint32_t ok = 0;                                         // bit 4 j + r: token 16 j + 4 g + r counts
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t b = (base + 16 * j) / a.block;
-            ks[j] = ksc[b] * a.scale2;
-            vs[j] = vsc[b];
-            uint32_t kp = 0x01010101u;
-            if (a.keep) kp = *(const uint32_t *)(a.keep + slot * a.keep_stride + base + 16 * j + 4 * g);
-#pragma unroll
             for (int r = 0; r < 4; r++)
-                if (base + 16 * j + 4 * g + r < len && ((kp >> (8 * r)) & 0xffu)) ok |= 1u << (4 * j + r);
-        }
+                if (base + 16 * j + 4 * g + r < len && ((x.keep[j] >> (8 * r)) & 0xffu)) ok |= 1u << (4 * j + r);
         f32x4 s[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -289,28 +324,32 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv8_attend(AttendArgs a)
 #pragma unroll
             for (int h = 0; h < HALVES; h++)
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const bf16x8 A = bytes8(kw[j][h][2 * x], kw[j][h][2 * x + 1]);
+                for (int i = 0; i < 2; i++) {
+                    const bf16x8 A = bytes8(x.k[j][h][2 * i], x.k[j][h][2 * i + 1]);
 #pragma unroll
-                    for (int n = 0; n < NQ; n++) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, q[h][x][n], s[j], 0, 0, 0);
+                    for (int n = 0; n < NQ; n++) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, q[h][i][n], s[j], 0, 0, 0);
                 }
         }
         float mx = m;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int j = 0; j < 4; j++) {
+            const float f = x.ks[j] * a.scale2;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                s[j][r] = (ok >> (4 * j + r)) & 1 ? s[j][r] * ks[j] : NINF;
+                s[j][r] = (ok >> (4 * j + r)) & 1 ? s[j][r] * f : NINF;
                 mx = fmaxf(mx, s[j][r]);
             }
+        }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float mu = mx == NINF ? 0.f : mx;                  // (nothing seen yet: every p below is exp2(-inf) = 0)
-        const float alpha = __builtin_amdgcn_exp2f(m - mu);
-        m = mx;
-        l *= alpha;
+        if (__any(mx != m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - mu);
+            l *= alpha;
 #pragma unroll
-        for (int d = 0; d < DT; d++) o[d] *= alpha;
+            for (int d = 0; d < DT; d++) o[d] *= alpha;
+        }
+        m = mx;
         float pv[16];
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -318,7 +357,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv8_attend(AttendArgs a)
             for (int r = 0; r < 4; r++) {
                 const float p = __builtin_amdgcn_exp2f(s[j][r] - mu);
                 l += p;
-                pv[4 * j + r] = (ok >> (4 * j + r)) & 1 ? p * vs[j] : 0.f;      // (a block behind the length may have any scale)
+                pv[4 * j + r] = (ok >> (4 * j + r)) & 1 ? p * x.vs[j] : 0.f;      // (a block behind the length may have any scale)
             }
         if (__any(ok != 0xffffu)) {
 #pragma unroll
@@ -326,20 +365,21 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv8_attend(AttendArgs a)
                 const uint32_t b = ok >> (4 * j);
                 const uint32_t mask = (b & 1 ? 0xffu : 0u) | (b & 2 ? 0xff00u : 0u) | (b & 4 ? 0xff0000u : 0u) | (b & 8 ? 0xff000000u : 0u);
 #pragma unroll
-                for (int d = 0; d < DT; d++) vw[d][j] &= mask;
+                for (int d = 0; d < DT; d++) v[d][j] &= mask;
             }
         }
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
+        for (int i = 0; i < 2; i++) {
             Planes pl;
-            split8(pv + 8 * x, pl);
+            split8(pv + 8 * i, pl);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const bf16x8 A = bytes8(vw[d][2 * x], vw[d][2 * x + 1]);
+                const bf16x8 A = bytes8(v[d][2 * i], v[d][2 * i + 1]);
 #pragma unroll
                 for (int n = 0; n < NP; n++) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, pl.p[n], o[d], 0, 0, 0);
             }
         }
+        if (WAVES > 1 && t < t_end) { load_v<DH>(vb, t, c, g, v); x = y; }
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -357,65 +397,162 @@ __global__ __launch_bounds__(64 * WAVES) void k_kv8_attend(AttendArgs a)
 #pragma unroll
         for (int w = 0; w < WAVES; w++) { f[w] = __builtin_amdgcn_exp2f(s_m[w][c] - mu); l += f[w] * s_l[w][c]; }
         m = mm;
-        for (uint32_t d = wave; d < DT; d += WAVES) {
-            f32x4 v = f[0] * s_o[0][d][lane];
 #pragma unroll
-            for (int w = 1; w < WAVES; w++) v += f[w] * s_o[w][d][lane];
-            s_o[0][d][lane] = v;                                 // (this wave's d alone)
+        for (int d = 0; d < DT; d += WAVES) {                    // (DT is a multiple of the waves: each joins its share of the dims)
+            f32x4 v = f[0] * s_o[0][d + wave][lane];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) v += f[w] * s_o[w][d + wave][lane];
+            o[d / WAVES] = v;
         }
     }
+    if (!live) return;
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);    // (nothing left: zeros; NaN stays)
-    if (a.splits == 1) {
-        if (!live) return;
-        T_ *out = (T_ *)a.out + (row * a.heads * a.share + hq) * DH;
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            if (WAVES > 1 && d % WAVES != wave) continue;
-            const f32x4 v = WAVES > 1 ? s_o[0][d][lane] : o[d];
-#pragma unroll
-            for (int r = 0; r < 4; r++) store1(out + 16 * d + 4 * g + r, v[r] * inv);
-        }
-        return;
+    float *part = nullptr;
+    T_ *out = (T_ *)a.out + (row * a.heads * a.share + hq) * DH;
+    if (a.splits > 1) {
+        part = a.part + (((uint64_t)sh * queries + qi) * a.splits + split) * (DH + 4);
+        if (wave == 0 && g == 0) { part[DH] = m; part[DH + 1] = l; }
     }
-    float *part = a.part + (((uint64_t)item * a.splits + split) * 16 + c) * (DH + 4);
-    if (wave == 0 && g == 0) { part[DH] = m; part[DH + 1] = l; }
 #pragma unroll
-    for (int d = 0; d < DT; d++) {
-        if (WAVES > 1 && d % WAVES != wave) continue;
-        *(f32x4 *)(part + 16 * d + 4 * g) = WAVES > 1 ? s_o[0][d][lane] : o[d];
+    for (int d = 0; d < DT / (WAVES > 1 ? WAVES : 1); d++) {
+        const uint32_t dim = 16 * (d * (WAVES > 1 ? WAVES : 1) + wave) + 4 * g;
+        if (part) *(f32x4 *)(part + dim) = o[d];
+        else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) store1(out + dim + r, o[d][r] * inv);
+        }
     }
 }
 
-// the parts of one (query row, query head) joined: one wave each
+// One query on a cache of one tile (a decode step over the short history of each of many rows): the matrix instructions would compute sixteen, and the registers of their
+// operands keep waves away that this case needs -- it is bound by the round trips of its loads, 300 rows x 16 heads being one wave each.  Plain
+// multiply-adds on the same loads: lane (g, c) has dims 16 g .. of token c of each sixteen, then tokens 4 g .. of dim c.
+template <typename T_, int DH>
+__global__ __launch_bounds__(256) void k_kv8_attend_one(AttendArgs a)
+{
+    enum { HALVES = DH / 64, DT = DH / 16 };
+    const float NINF = -__builtin_huge_valf();
+    __shared__ __attribute__((aligned(16))) float s_p[4][64];
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15, g = lane >> 4;
+    const uint32_t sh = blockIdx.x * 4 + wave;
+    if (sh >= a.items) return;
+    const uint32_t slot = sh / a.heads, head = sh % a.heads;
+    const uint8_t *kb = a.k + (uint64_t)sh * 64 * DH, *vb = a.v + (uint64_t)sh * 64 * DH;
+    const float *ksc = a.k_scale + (uint64_t)sh * (64 / a.block), *vsc = a.v_scale + (uint64_t)sh * (64 / a.block);
+    const uint8_t *keep = a.keep ? a.keep + slot * a.keep_stride : nullptr;
+    u32x4 v[DT];
+    load_v<DH>(vb, 0, c, g, v);
+    float q[16 * HALVES];
+#pragma unroll
+    for (int h = 0; h < HALVES; h++) load16((const T_ *)a.q + slot * a.q_row + (uint64_t)head * a.q_head + 64 * h + 16 * g, a.vec, q + 16 * h);
+    const int32_t raw = a.lengths[slot];
+    const uint32_t len = raw < 0 ? 0 : min((uint32_t)raw, 64u);
+    u32x4 k[4][HALVES];
+    float s[4], m = NINF;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (16 * j < (int)len) {
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) k[j][h] = *(const u32x4 *)(kb + (16 * j + c) * DH + 64 * h + 16 * g);
+        }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        s[j] = NINF;
+        if (16 * j >= (int)len) continue;
+        float acc = 0.f;
+#pragma unroll
+        for (int h = 0; h < HALVES; h++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)k[j][h][w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)k[j][h][w], true);
+                const float *x = q + 16 * h + 4 * w;
+                acc = fmaf(lo[0], x[0], acc); acc = fmaf(lo[1], x[1], acc); acc = fmaf(hi[0], x[2], acc); acc = fmaf(hi[1], x[3], acc);
+            }
+        acc += __shfl_xor(acc, 16);
+        acc += __shfl_xor(acc, 32);
+        const uint32_t t = 16 * j + c;
+        if (t < len && (!keep || keep[t])) s[j] = acc * (ksc[16 * j / a.block] * a.scale2);
+        m = fmaxf(m, s[j]);
+    }
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float mu = m == NINF ? 0.f : m;
+    float l = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float p = __builtin_amdgcn_exp2f(s[j] - mu);
+        l += p;
+        if (g == 0) s_p[wave][16 * j + c] = s[j] == NINF ? 0.f : p * vsc[16 * j / a.block];       // (a block behind the length may have any scale)
+    }
+    for (int o = 8; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");       // (the wave's own: its LDS operations stay in order)
+    float o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (16 * j >= (int)len) continue;
+        const f32x4 p = *(const f32x4 *)&s_p[wave][16 * j + 4 * g];
+        // (bytes of tokens that do not count may be NaN)
+        uint32_t mask = 0xffffffffu;
+        const int left = (int)len - (16 * j + 4 * (int)g);
+        if (left < 4) mask = left <= 0 ? 0u : mask >> (8 * (4 - left));
+        if (keep) {
+            const uint32_t kp = *(const uint32_t *)(keep + 16 * j + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++) if (!((kp >> (8 * r)) & 0xffu)) mask &= ~(0xffu << (8 * r));
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const uint32_t w = v[d][j] & mask;
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+            o[d] = fmaf(lo[0], p[0], o[d]); o[d] = fmaf(lo[1], p[1], o[d]); o[d] = fmaf(hi[0], p[2], o[d]); o[d] = fmaf(hi[1], p[3], o[d]);
+        }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    T_ *out = (T_ *)a.out + (uint64_t)sh * DH;
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        o[d] += __shfl_xor(o[d], 16);
+        o[d] += __shfl_xor(o[d], 32);
+        if ((d & 3) == (int)g) store1(out + 16 * d + c, o[d] * inv);
+    }
+}
+
+// the parts of one (query row, query head) joined: a workgroup, whose waves take the parts in turn
 template <typename T_, int DH>
 __global__ __launch_bounds__(256) void k_kv8_join(AttendArgs a)
 {
+    enum { H = DH / 64 };
     const float NINF = -__builtin_huge_valf();
-    const uint32_t lane = threadIdx.x & 63;
-    const uint64_t id = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t queries = a.beams * a.share;
-    if (id >= (uint64_t)a.slots * a.heads * queries) return;
-    const uint32_t qi = (uint32_t)(id % queries), sh = (uint32_t)(id / queries), slot = sh / a.heads, head = sh % a.heads;
-    const float *part = a.part + (((uint64_t)sh * a.qtiles + qi / 16) * a.splits * 16 + qi % 16) * (DH + 4);
-    const uint64_t step = (uint64_t)16 * (DH + 4);
+    __shared__ float s_l[4], s_v[4][DH];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t id = blockIdx.x;
+    const uint32_t queries = a.beams * a.share, qi = (uint32_t)(id % queries), sh = (uint32_t)(id / queries), slot = sh / a.heads, head = sh % a.heads;
+    const float *part = a.part + id * a.splits * (DH + 4);
     float m = NINF;
-    for (uint32_t s = lane; s < a.splits; s += 64) m = fmaxf(m, part[s * step + DH]);
+    for (uint32_t s = lane; s < a.splits; s += 64) m = fmaxf(m, part[s * (uint64_t)(DH + 4) + DH]);
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const float mu = m == NINF ? 0.f : m;
-    float l = 0.f, v[DH / 64];
+    float l = 0.f, v[H];
 #pragma unroll
-    for (int h = 0; h < DH / 64; h++) v[h] = 0.f;
-    for (uint32_t s = 0; s < a.splits; s++) {
-        const float f = __builtin_amdgcn_exp2f(part[s * step + DH] - mu);
-        l += f * part[s * step + DH + 1];
+    for (int h = 0; h < H; h++) v[h] = 0.f;
+#pragma unroll 4
+    for (uint32_t s = wave; s < a.splits; s += 4) {
+        const float *p = part + s * (uint64_t)(DH + 4);
+        const float f = __builtin_amdgcn_exp2f(p[DH] - mu);
+        l += f * p[DH + 1];
 #pragma unroll
-        for (int h = 0; h < DH / 64; h++) v[h] += f * part[s * step + 64 * h + lane];
+        for (int h = 0; h < H; h++) v[h] += f * p[64 * h + lane];
     }
+    if (lane == 0) s_l[wave] = l;
+#pragma unroll
+    for (int h = 0; h < H; h++) s_v[wave][64 * h + lane] = v[h];
+    __syncthreads();
+    l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     const uint64_t row = (uint64_t)slot * a.beams + qi / a.share;
     T_ *out = (T_ *)a.out + (row * a.heads * a.share + head * a.share + qi % a.share) * DH;
-#pragma unroll
-    for (int h = 0; h < DH / 64; h++) store1(out + 64 * h + lane, v[h] * inv);
+    if (threadIdx.x < DH) store1(out + threadIdx.x, (s_v[0][threadIdx.x] + s_v[1][threadIdx.x] + s_v[2][threadIdx.x] + s_v[3][threadIdx.x]) * inv);
 }
 
 // ---- C ABI ----
@@ -465,10 +602,10 @@ static int kv8_append(void *stream, const void *k_new, const void *v_new, const 
 template <typename T_, int DH>
 static void launch_attend(hipStream_t st, const AttendArgs &a)
 {
-    const uint32_t grid = a.slots * a.heads * a.qtiles * a.splits;
-    if (a.T == 64) hipLaunchKernelGGL((k_kv8_attend<T_, DH, 1>), dim3(grid), dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((k_kv8_attend<T_, DH, 4>), dim3(grid), dim3(256), 0, st, a);
-    if (a.splits > 1) hipLaunchKernelGGL((k_kv8_join<T_, DH>), dim3((uint32_t)(((uint64_t)a.slots * a.heads * a.beams * a.share + 3) / 4)), dim3(256), 0, st, a);
+    if (a.T == 64 && a.beams * a.share == 1) hipLaunchKernelGGL((k_kv8_attend_one<T_, DH>), dim3((a.items + 3) / 4), dim3(256), 0, st, a);
+    else if (a.T == 64) hipLaunchKernelGGL((k_kv8_attend<T_, DH, 1>), dim3((a.items + 3) / 4), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_kv8_attend<T_, DH, 4>), dim3(a.items * a.splits), dim3(256), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL((k_kv8_join<T_, DH>), dim3(a.slots * a.heads * a.beams * a.share), dim3(256), 0, st, a);
 }
 
 template <typename T_>
@@ -491,14 +628,16 @@ static int kv8_attend(void *stream, const void *q, uint64_t q_row_stride, uint64
     a.out = out; a.part = (float *)work;
     a.slots = slots; a.heads = heads; a.share = share; a.beams = beams; a.T = T; a.block = block; a.splits = splits;
     const uint64_t queries = (uint64_t)beams * share, qtiles = (queries + 15) / 16, items = (uint64_t)slots * heads * qtiles;
-    if (queries > (1u << 20) || items * splits > 0x7fffffffull || (uint64_t)slots * heads * queries > 0xfffffff0ull) {
+    if (queries > (1u << 20) || items * splits > 0x7fffffffull || (uint64_t)slots * heads * queries > 0x7fffffffull) {
         fmi_set_error("sealnn_kv8_attend: %u slots x %u heads x %llu queries are too many", slots, heads, (unsigned long long)queries);
         return FMI_ERR_UNSUPPORTED;
     }
     a.qtiles = (uint32_t)qtiles;
+    a.items = (uint32_t)items;
+    a.vec = (((uintptr_t)q | q_row_stride * sizeof(T_) | q_head_stride * sizeof(T_)) & 15) == 0;
     a.scale2 = scale * 1.4426950408889634f;
-    if (splits > 1 && (!work || ((uintptr_t)work & 15) || work_bytes < items * splits * 16 * (dh + 4) * sizeof(float))) {
-        fmi_set_error("sealnn_kv8_attend: the workspace must hold %llu bytes", (unsigned long long)(items * splits * 16 * (dh + 4) * sizeof(float)));
+    if (splits > 1 && (!work || ((uintptr_t)work & 15) || work_bytes < (uint64_t)slots * heads * queries * splits * (dh + 4) * sizeof(float))) {
+        fmi_set_error("sealnn_kv8_attend: the workspace must hold %llu bytes", (unsigned long long)((uint64_t)slots * heads * queries * splits * (dh + 4) * sizeof(float)));
         return FMI_ERR_CAPACITY;
     }
     if (dh == 64) launch_attend<T_, 64>((hipStream_t)stream, a);

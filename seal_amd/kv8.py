@@ -11,7 +11,9 @@ import torch
 from ._lib import launch, lib, uint64s
 
 TILE = 64                                  # tokens of a tile of the layout
-WAVES_WANTED = 4096                        # waves that keep the memory of 256 CUs busy
+# Workgroups (of four waves) that a call splits long slots into when it has few: one a CU is enough for many items (32 slots x 8 heads of up to 8192 tokens: 79 us, in two
+# parts 84), two a CU are better where every item is split anyway (1 slot x 16 heads of 32001 tokens: 16 parts 19.0 us, 32 18.0, 64 19.3)
+ITEMS_ENOUGH, PARTS_WANTED = 256, 512
 
 
 class KV8Cache:
@@ -99,10 +101,10 @@ class KV8Cache:
         lengths_ptr, index = self._lengths(lengths, "lengths"), self._on_gpu()
         out = q.new_empty(shape)
         items = self.slots * H * ((beams * share + 15) // 16)
-        splits = max(1, min(self.tokens // TILE // 4, WAVES_WANTED // 4 // max(items, 1)))
+        splits = 1 if items >= ITEMS_ENOUGH or not items else max(1, min(self.tokens // TILE // 4, PARTS_WANTED // items))
         work, work_floats = None, 0
         if splits > 1:
-            work_floats = items * splits * 16 * (D + 4)
+            work_floats = shape[0] * shape[1] * splits * (D + 4)
             work = torch.empty(work_floats, dtype=torch.float32, device=self.device)
         launch(lib().sealnn_kv8_attend if dt == torch.float32 else lib().sealnn_kv8_attend_bf16, index, q.data_ptr(), row_stride, head_stride, self.k.data_ptr(),
                self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), lengths_ptr, keep_ptr, keep_stride, self.slots, beams, H, share, self.tokens,

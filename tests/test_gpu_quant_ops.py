@@ -287,11 +287,11 @@ def test_attend_strided_queries_scale_and_parts():
     exact, mag, vmax = ref.attend(q.double().cpu().numpy(), k.values(), v.values(), ln.tolist(), beams)
     from seal_amd import kv8
     for wanted in (1, 1 << 14):
-        old, kv8.WAVES_WANTED = kv8.WAVES_WANTED, wanted
+        old, kv8.PARTS_WANTED = kv8.PARTS_WANTED, wanted
         try:
             got = c.attend(q, ln, beams=beams).double().cpu().numpy()
         finally:
-            kv8.WAVES_WANTED = old
+            kv8.PARTS_WANTED = old
         assert (np.abs(got - exact) <= _attend_bound(mag, T, exact, D, vmax, F32)).all()
 
 
