@@ -22,12 +22,14 @@ static __device__ __forceinline__ int exponent_for(float amax)
     const float m = frexpf(amax, &x);
     return amax > 0.f ? max(x - (m <= 0.875f ? 9 : 8), (int)E_MIN) : (int)E_MIN;
 }
-// four numbers, already divided by the scale, as e4m3 codes: to nearest, ties to even; infinities become +-448, NaN stays
+// Four numbers, already divided by the scale, as e4m3 codes: to nearest, ties to even; NaN stays.  A block's scale holds its finite values (the instruction alone does
+// then); with `wild` there may be infinities, which become +-448.
 static __device__ __forceinline__ float sat(float y) { return y != y ? y : fminf(fmaxf(y, -448.f), 448.f); }
-static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d)
+static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, bool wild = false)
 {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(sat(a), sat(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(sat(c), sat(d), w, true);
+    if (wild) { a = sat(a); b = sat(b); c = sat(c); d = sat(d); }
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 // four codes times 2^shift (shift <= 0), re-encoded
 static __device__ __forceinline__ uint32_t shift4(uint32_t w, float f)
@@ -71,99 +73,231 @@ static __device__ __forceinline__ void load16(const T_ *p, bool vec, float v[16]
     }
 }
 
-// One workgroup of NTHR threads per (slot, head, 64-token tile, K or V).  Nobody else writes the tile, so bytes that the call does not
-// touch are carried over by reading them.  First the largest magnitude of the new tokens of each block, then the codes.
-template <typename T_, int NTHR>
-__global__ __launch_bounds__(NTHR) void k_kv8_append(AppendArgs a, uint32_t vec)
+static __device__ __forceinline__ float larger(float m, float v) { return fmaxf(m, fabsf(v)); }                      // (NaN is left out)
+static __device__ __forceinline__ float larger_finite(float m, float v) { return fabsf(v) < __builtin_huge_valf() ? fmaxf(m, fabsf(v)) : m; }
+static __device__ __forceinline__ float wave_largest(float m)
 {
-    __shared__ uint32_t s_max[4];
-    __shared__ __attribute__((aligned(16))) uint8_t s_tile[128 * 80];     // V: [dh][64 tokens + padding]
-    const uint32_t which = blockIdx.z, slot = blockIdx.y / a.heads, head = blockIdx.y % a.heads, tid = threadIdx.x;
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    return m;
+}
+
+// One new token (a decode step): a wave per (slot, head), a lane per dim (two for 128).  The codes of the block before it are only touched where its scale has to grow.
+template <typename T_, int DH>
+__global__ __launch_bounds__(256) void k_kv8_append_one(AppendArgs a)
+{
+    enum { N = DH / 64 };
+    const uint32_t lane = threadIdx.x & 63, sh = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (sh >= a.slots * a.heads) return;
+    const uint32_t slot = sh / a.heads, head = sh % a.heads, blk = a.block;
+    float x[2][N], m[2];
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        const T_ *src = (const T_ *)a.src[w] + slot * a.slot_stride[w] + head * a.head_stride[w];
+        m[w] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) x[w][i] = load1(src + 64 * i + lane);
+    }
+    const int32_t len = a.lengths[slot];
+    if (len < 0 || len >= (int32_t)a.T || (a.counts && a.counts[slot] <= 0)) return;
+    const uint32_t t = (uint32_t)len % 64, held = (uint32_t)len % blk;                // place in the tile; tokens that the block holds
+    const uint64_t tile = (uint32_t)len / 64;
+    float *scale[2] = {a.scale[0] + (uint64_t)sh * (a.T / blk) + (uint32_t)len / blk, a.scale[1] + (uint64_t)sh * (a.T / blk) + (uint32_t)len / blk};
+    int e_old[2], e[2];
+    if (held) { e_old[0] = exponent_of(*scale[0]); e_old[1] = exponent_of(*scale[1]); }
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+#pragma unroll
+        for (int i = 0; i < N; i++) m[w] = larger_finite(m[w], x[w][i]);
+        e[w] = exponent_for(wave_largest(m[w]));
+        if (held) e[w] = max(e[w], e_old[w]);
+    }
+    uint8_t *k = a.codes[0] + ((uint64_t)sh * a.T + tile * 64) * DH, *v = a.codes[1] + ((uint64_t)sh * a.T + tile * 64) * DH;
+    if (held && e[0] > e_old[0]) {
+        const float f = pow2i(max(e_old[0] - e[0], -126));
+        for (uint32_t u = lane; u < held * (DH / 16); u += 64) {
+            u32x4 *p = (u32x4 *)(k + (uint64_t)(t - held) * DH + 16 * u);
+            u32x4 w = *p;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = shift4(w[i], f);
+            *p = w;
+        }
+    }
+    if (held && e[1] > e_old[1]) {
+        const float f = pow2i(max(e_old[1] - e[1], -126));
+        for (uint32_t u = lane; u < DH * 4; u += 64) {           // 16 bytes: dim u / 4, tokens 16 j + 4 (u % 4) + r
+            u32x4 *p = (u32x4 *)(v + 16 * u);
+            u32x4 w = *p;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                uint32_t mask = 0;
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) { const uint32_t s = 16 * j + 4 * (u % 4) + r; if (s >= t - held && s < t) mask |= 0xffu << (8 * r); }
+                w[j] = (w[j] & ~mask) | (shift4(w[j], f) & mask);
+            }
+            *p = w;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (the new token's bytes below go on top of these words)
+        __builtin_amdgcn_s_waitcnt(0);
+    }
+    if (lane < 2) *(lane ? scale[1] : scale[0]) = pow2i(lane ? e[1] : e[0]);
+    const uint32_t at = ((t >> 2) & 3) * 16 + (t >> 4) * 4 + (t & 3);
+    const float f0 = pow2i(-e[0]), f1 = pow2i(-e[1]);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t w = encode4(x[0][i] * f0, x[1][i] * f1, 0.f, 0.f, true);
+        k[(uint64_t)t * DH + 64 * i + lane] = (uint8_t)w;
+        v[(uint64_t)(64 * i + lane) * 64 + at] = (uint8_t)(w >> 8);
+    }
+}
+
+// Many new tokens: a workgroup of 256 threads per (slot, head, 64-token tile).  Nobody else writes the tile, so bytes that the call does not touch are carried over by
+// reading them.  K and V together -- what limits the call is how many loads a CU has on their way --, held from the search for the blocks' largest
+// magnitudes to the codes.  K: a thread has sixteen dims of a token, 16 bytes of its row.  V: four dims of four tokens -- the four tokens' codes of a
+// dim are a word of its row, turned round in LDS (swizzled: 64 lanes, 64 banks).
+template <typename T_, int DH>
+__global__ __launch_bounds__(256) void k_kv8_append(AppendArgs a, uint32_t vec)
+{
+    enum { N = DH / 64, PITCH = 20 };                            // words of a row of V in LDS
+    __shared__ uint32_t s_max[2][4];
+    __shared__ uint32_t s_tile[DH * PITCH];
+    // (the heads of a tile next to each other: their values are neighbours in memory)
+    const uint32_t head = blockIdx.x % a.heads, slot = blockIdx.y, tid = threadIdx.x;
     const int64_t len = a.lengths[slot];
     const int64_t cnt = a.counts ? min((int64_t)a.counts[slot], (int64_t)a.n) : (int64_t)a.n;
     if (len < 0 || len >= (int64_t)a.T || cnt <= 0) return;
-    const int64_t tile = len / 64 + blockIdx.x, base = tile * 64;
+    const int64_t tile = len / 64 + blockIdx.x / a.heads, base = tile * 64;
     const int64_t lo = max(len, base), hi = min(min(len + cnt, (int64_t)a.T), base + 64);
     if (lo >= hi) return;
     const uint32_t l0 = (uint32_t)(lo - base), l1 = (uint32_t)(hi - base);           // new tokens of the tile
-    const uint32_t dh = a.dh, chunks = dh / 16, blk = a.block;
+    const uint32_t blk = a.block, t_own = tid / 4, tq = tid / 16;
     const uint64_t sh = (uint64_t)slot * a.heads + head;
-    const T_ *src = (const T_ *)a.src[which] + slot * a.slot_stride[which] + head * a.head_stride[which];
-    float *scale = a.scale[which] + sh * (a.T / blk) + (uint64_t)base / blk;
-    if (tid < 4) s_max[tid] = 0;
-    __syncthreads();
-    for (uint32_t u = tid; u < (l1 - l0) * chunks; u += NTHR) {
-        const uint32_t t = l0 + u / chunks, c = u % chunks;
-        float v[16], m = 0.f;
-        load16(src + (uint64_t)(base + t - len) * a.token_stride[which] + 16 * c, vec, v);
+    float x[2][N][4][4];                                         // K: [half][run of four dims][dim] of token t_own; V: [half][token 4 tq + r][dim]
+    {
+        // every load first, then what is done with the values (a thread without a token of the call reads the first one's)
+        typedef typename std::conditional<std::is_same<T_, float>::value, f32x4, u32x2>::type Raw;
+        const T_ *p[2][4];
+        Raw raw[2][N][4];
 #pragma unroll
-        for (int i = 0; i < 16; i++) m = fabsf(v[i]) < __builtin_huge_valf() ? fmaxf(m, fabsf(v[i])) : m;
-        atomicMax(&s_max[t / blk], as_u32(m));                   // (magnitudes order as their bits: the same whatever the order)
-    }
-    __syncthreads();
-    // the blocks of this tile that the call touches, their old and new exponents
-    const uint32_t b0 = l0 / blk, b1 = (l1 - 1) / blk;
-    const bool held = l0 % blk != 0;                             // the first touched block had tokens before
-    int e_new[4], e_old = 0;
+        for (int w = 0; w < 2; w++)
 #pragma unroll
-    for (uint32_t b = 0; b < 4; b++) e_new[b] = (b >= b0 && b <= b1) ? exponent_for(as_f32(s_max[b])) : 0;
-    if (held) {
-        e_old = exponent_of(scale[b0]);
-        e_new[0] = b0 == 0 ? max(e_new[0], e_old) : e_new[0]; e_new[1] = b0 == 1 ? max(e_new[1], e_old) : e_new[1];
-        e_new[2] = b0 == 2 ? max(e_new[2], e_old) : e_new[2]; e_new[3] = b0 == 3 ? max(e_new[3], e_old) : e_new[3];
-    }
-    auto exp_of = [&](uint32_t b) { return b == 0 ? e_new[0] : b == 1 ? e_new[1] : b == 2 ? e_new[2] : e_new[3]; };
-    const int e_held = exp_of(b0);
-    const bool grow = held && e_held > e_old;
-    const float shift = grow ? pow2i(max(e_old - e_held, -126)) : 1.f;
-    __syncthreads();                                             // (every thread has read the old scale)
-    if (tid < 4 && tid >= b0 && tid <= b1) scale[tid] = pow2i(exp_of(tid));
-    if (which == 0) {
-        uint8_t *codes = a.codes[0] + (sh * a.T + (uint64_t)base) * dh;
-        for (uint32_t u = tid; u < (l1 - l0) * chunks; u += NTHR) {
-            const uint32_t t = l0 + u / chunks, c = u % chunks;
-            float v[16];
-            load16(src + (uint64_t)(base + t - len) * a.token_stride[which] + 16 * c, vec, v);
-            const float f = pow2i(-exp_of(t / blk));
-            u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = encode4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f);
-            *(u32x4 *)(codes + (uint64_t)t * dh + 16 * c) = w;
-        }
-        if (grow)
-            for (uint32_t u = tid; u < (l0 - b0 * blk) * chunks; u += NTHR) {
-                u32x4 *p = (u32x4 *)(codes + (uint64_t)(b0 * blk + u / chunks) * dh + 16 * (u % chunks));
-                u32x4 w = *p;
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = shift4(w[i], shift);
-                *p = w;
+            for (uint32_t r = 0; r < 4; r++) {
+                const uint32_t t = w ? 4 * tq + r : t_own;
+                p[w][r] = (const T_ *)a.src[w] + slot * a.slot_stride[w] + head * a.head_stride[w] + (w ? tid % 16 * 4 : tid % 4 * 16 + 4 * r) +
+                          (uint64_t)(base + (t >= l0 && t < l1 ? t : l0) - len) * a.token_stride[w];
             }
-        return;
+        if (vec) {
+#pragma unroll
+            for (int w = 0; w < 2; w++)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) raw[w][i][r] = *(const Raw *)(p[w][r] + 64 * i);
+        } else {
+#pragma unroll
+            for (int w = 0; w < 2; w++)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const T_ *q = p[w][r] + 64 * i;
+                        if constexpr (std::is_same<T_, float>::value) raw[w][i][r] = f32x4{q[0], q[1], q[2], q[3]};
+                        else { const uint16_t *h = (const uint16_t *)q; raw[w][i][r] = u32x2{(uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16)}; }
+                    }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++) {
+                const uint32_t t = w ? 4 * tq + r : t_own;
+                const bool live = t >= l0 && t < l1;
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        if constexpr (std::is_same<T_, float>::value) x[w][i][r][d] = live ? raw[w][i][r][d] : 0.f;
+                        else x[w][i][r][d] = live ? as_f32(d & 1 ? raw[w][i][r][d / 2] & 0xffff0000u : raw[w][i][r][d / 2] << 16) : 0.f;
+                    }
+            }
     }
-    // V: the codes of the new tokens transposed through LDS, then merged into the tile's rows
-    for (uint32_t u = tid; u < (l1 - l0) * chunks; u += NTHR) {
-        const uint32_t t = l0 + u / chunks, c = u % chunks;
-        float v[16];
-        load16(src + (uint64_t)(base + t - len) * a.token_stride[which] + 16 * c, vec, v);
-        const float f = pow2i(-exp_of(t / blk));
-        const uint32_t at = ((t >> 2) & 3) * 16 + (t >> 4) * 4 + (t & 3);
+    // the blocks of this tile that the call touches; the first of them may have had tokens before
+    const uint32_t b0 = l0 / blk, b1 = (l1 - 1) / blk;
+    const bool held = l0 % blk != 0;
+    float *scale[2];
+    int e_old[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t w = encode4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f);
+    for (int w = 0; w < 2; w++) {
+        scale[w] = a.scale[w] + sh * (a.T / blk) + (uint64_t)base / blk;
+        if (held) e_old[w] = exponent_of(scale[w][b0]);
+    }
+    if (tid < 8) s_max[tid / 4][tid % 4] = 0;
+    float m[2];
+    bool wild[2];
 #pragma unroll
-            for (int j = 0; j < 4; j++) s_tile[(16 * c + 4 * i + j) * 80 + at] = (uint8_t)(w >> (8 * j));
+    for (int w = 0; w < 2; w++) {
+        m[w] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16 * N; i++) m[w] = larger(m[w], x[w][i / 16][i / 4 % 4][i % 4]);
+        m[w] = wave_largest(m[w]);                               // (a wave has sixteen tokens: of one block)
+        wild[w] = !(m[w] < __builtin_huge_valf());               // infinities do not count
+        if (wild[w]) {
+            m[w] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16 * N; i++) m[w] = larger_finite(m[w], x[w][i / 16][i / 4 % 4][i % 4]);
+            m[w] = wave_largest(m[w]);
         }
     }
     __syncthreads();
-    uint8_t *codes = a.codes[1] + (sh * a.T + (uint64_t)base) * dh;
+    if ((tid & 63) == 0) { atomicMax(&s_max[0][t_own / blk], as_u32(m[0])); atomicMax(&s_max[1][t_own / blk], as_u32(m[1])); }     // (magnitudes order as their bits)
+    __syncthreads();
+    auto exp_of = [&](int w, uint32_t b) { const int e = exponent_for(as_f32(s_max[w][b])); return held && b == b0 ? max(e, e_old[w]) : e; };
+    float f[2], shift[2];
+    bool grow[2];
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        const int e = exp_of(w, b0);
+        grow[w] = held && e > e_old[w];
+        shift[w] = grow[w] ? pow2i(max(e_old[w] - e, -126)) : 1.f;
+        f[w] = pow2i(-exp_of(w, t_own / blk));                   // (4 tq and t_own are of the same sixteen tokens)
+        if (tid >= b0 && tid <= b1) scale[w][tid] = pow2i(exp_of(w, tid));           // (every thread has read the old scale: two barriers ago)
+    }
+    uint8_t *k = a.codes[0] + (sh * a.T + (uint64_t)base) * DH, *v = a.codes[1] + (sh * a.T + (uint64_t)base) * DH;
+    if (t_own >= l0 && t_own < l1) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            u32x4 c;
+#pragma unroll
+            for (int r = 0; r < 4; r++) c[r] = encode4(x[0][i][r][0] * f[0], x[0][i][r][1] * f[0], x[0][i][r][2] * f[0], x[0][i][r][3] * f[0], wild[0]);
+            *(u32x4 *)(k + (uint64_t)t_own * DH + 64 * i + tid % 4 * 16) = c;
+        }
+    }
+    if (grow[0])
+        for (uint32_t u = tid; u < (l0 - b0 * blk) * (DH / 16); u += 256) {
+            u32x4 *p = (u32x4 *)(k + (uint64_t)(b0 * blk) * DH + 16 * u);
+            u32x4 c = *p;
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = shift4(c[i], shift[0]);
+            *p = c;
+        }
+    // V: row d, word 4 g + j (tokens 16 j + 4 g .. + 3, tq = 4 j + g) stands at word (4 g + j + d / 16) % 16
+    const uint32_t col = 4 * (tq & 3) + (tq >> 2);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+            const uint32_t row = 64 * i + tid % 16 * 4 + d;
+            s_tile[row * PITCH + ((col + row / 16) & 15)] = encode4(x[1][i][0][d] * f[1], x[1][i][1][d] * f[1], x[1][i][2][d] * f[1], x[1][i][3][d] * f[1], wild[1]);
+        }
+    __syncthreads();
     const bool whole = l0 == 0 && l1 == 64;
-    for (uint32_t u = tid; u < dh * 4; u += NTHR) {
+    for (uint32_t u = tid; u < DH * 4; u += 256) {
         const uint32_t d = u / 4, g = u % 4;
-        u32x4 *p = (u32x4 *)(codes + (uint64_t)d * 64 + g * 16);
-        const u32x4 fresh = *(const u32x4 *)(s_tile + d * 80 + g * 16);
-        u32x4 w = fresh;
+        u32x4 *p = (u32x4 *)(v + 16 * u);
+        u32x4 fresh, c;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) fresh[j] = s_tile[d * PITCH + ((4 * g + j + d / 16) & 15)];
+        c = fresh;
         if (!whole) {
-            w = *p;
+            c = *p;
 #pragma unroll
             for (uint32_t j = 0; j < 4; j++) {                   // word j: tokens 16 j + 4 g .. + 3
                 const uint32_t t0 = 16 * j + 4 * g;
@@ -173,11 +307,11 @@ __global__ __launch_bounds__(NTHR) void k_kv8_append(AppendArgs a, uint32_t vec)
                     if (t0 + r >= l0 && t0 + r < l1) m_new |= 0xffu << (8 * r);
                     if (t0 + r >= b0 * blk && t0 + r < l0) m_old |= 0xffu << (8 * r);
                 }
-                const uint32_t again = grow ? shift4(w[j], shift) : w[j];
-                w[j] = (w[j] & ~(m_new | m_old)) | (again & m_old) | (fresh[j] & m_new);
+                const uint32_t again = grow[1] ? shift4(c[j], shift[1]) : c[j];
+                c[j] = (c[j] & ~(m_new | m_old)) | (again & m_old) | (fresh[j] & m_new);
             }
         }
-        *p = w;
+        *p = c;
     }
 }
 
@@ -579,7 +713,10 @@ static int kv8_append(void *stream, const void *k_new, const void *v_new, const 
         fmi_set_error("sealnn_kv8_append: the new tokens, their strides and the lengths must be given");
         return FMI_ERR_ARG;
     }
-    if ((uint64_t)slots * heads > 65535u) { fmi_set_error("sealnn_kv8_append: %u slots x %u heads are more than 65535", slots, heads); return FMI_ERR_UNSUPPORTED; }
+    if (slots > 65535u || (uint64_t)slots * heads > 0x7fffffffu || ((uint64_t)std::min(n, T) / 64 + 2) * heads > 0x7fffffffu) {
+        fmi_set_error("sealnn_kv8_append: %u slots (up to 65535) x %u heads x %u tokens are too many", slots, heads, n);
+        return FMI_ERR_UNSUPPORTED;
+    }
     AppendArgs a;
     a.src[0] = k_new; a.src[1] = v_new;
     uint64_t odd = (uintptr_t)k_new | (uintptr_t)v_new;
@@ -591,10 +728,17 @@ static int kv8_append(void *stream, const void *k_new, const void *v_new, const 
     a.scale[0] = k_scale; a.scale[1] = v_scale;
     a.lengths = lengths; a.counts = counts;
     a.n = std::min(n, T); a.slots = slots; a.heads = heads; a.T = T; a.block = block; a.dh = dh;
-    const uint32_t vec = (odd & 15) == 0;
-    const dim3 grid((a.n + 62) / 64 + 1, slots * heads, 2);
-    if (n == 1) hipLaunchKernelGGL((k_kv8_append<T_, 64>), grid, dim3(64), 0, (hipStream_t)stream, a, vec);
-    else hipLaunchKernelGGL((k_kv8_append<T_, 256>), grid, dim3(256), 0, (hipStream_t)stream, a, vec);
+    const uint32_t vec = (odd & (4 * sizeof(T_) - 1)) == 0;
+    const hipStream_t st = (hipStream_t)stream;
+    if (n == 1) {
+        const dim3 grid((slots * heads + 3) / 4);
+        if (dh == 64) hipLaunchKernelGGL((k_kv8_append_one<T_, 64>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_kv8_append_one<T_, 128>), grid, dim3(256), 0, st, a);
+    } else {
+        const dim3 grid(((a.n + 62) / 64 + 1) * heads, slots);
+        if (dh == 64) hipLaunchKernelGGL((k_kv8_append<T_, 64>), grid, dim3(256), 0, st, a, vec);
+        else hipLaunchKernelGGL((k_kv8_append<T_, 128>), grid, dim3(256), 0, st, a, vec);
+    }
     NNCHK();
     return FMI_OK;
 }
