@@ -186,13 +186,17 @@ int sealnn_kv8_attend_bf16(void *stream, const void *q, uint64_t q_row_stride, u
  *   have at least min_p of the largest weight (<= 0: off).
  * temperature <= 0: the first of the largest.  The *_v arrays ([rows], or NULL) override the numbers row by row.  NaN logits are never drawn, +inf counts as the
  * largest fp32 number.  tokens / logprobs [rows][draws]: -1 / -inf for a row without a token; logprobs = logit - logsumexp(row), neither
- * temperature nor filters applied. */
+ * temperature nor filters applied.
+ * work: NULL, and a workgroup does a row; or rows * (96 * ceil(vocab / 1024) + 16448) bytes, 16-byte aligned (at most 65535 rows of at least 4), and
+ * three kernels spread each row over the card, which pays for few rows of a large vocabulary.  The tokens are the same. */
 int sealnn_sample_tokens(void *stream, const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float *u, uint32_t draws,
                          const uint32_t *bits, uint64_t bits_stride, float temperature, int32_t top_k, float top_p, float min_p,
-                         const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs);
+                         const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs,
+                         void *work, uint64_t work_bytes);
 int sealnn_sample_tokens_bf16(void *stream, const void *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float *u, uint32_t draws,
                               const uint32_t *bits, uint64_t bits_stride, float temperature, int32_t top_k, float top_p, float min_p,
-                              const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs);
+                              const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs,
+                              void *work, uint64_t work_bytes);
 
 #ifdef __cplusplus
 }

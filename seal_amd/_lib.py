@@ -177,7 +177,8 @@ for _name, _args in (("w4_linear", [_vp, _vp, _u64, _vp, _vp, _vp, _u32, _u32, _
                      ("kv8_append", [_vp, _vp, _vp, _p64, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32]),
                      ("kv8_attend", [_vp, _vp, _u64, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _f32,
                                      _u32, _vp, _u64, _vp]),
-                     ("sample_tokens", [_vp, _vp, _u64, _u32, _u32, _vp, _u32, _vp, _u64, _f32, ctypes.c_int32, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _vp])):
+                     ("sample_tokens", [_vp, _vp, _u64, _u32, _u32, _vp, _u32, _vp, _u64, _f32, ctypes.c_int32, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                        _vp, _u64])):
     NN_SIGNATURES["sealnn_" + _name] = NN_SIGNATURES["sealnn_" + _name + "_bf16"] = (_int, _args)
 
 _lib = None

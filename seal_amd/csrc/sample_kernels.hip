@@ -26,6 +26,27 @@ struct SampleArgs {
     int32_t top_k;
     int64_t *tokens;
     float *logprobs;
+    char *work;                                                  // NULL: one kernel
+};
+
+// What the kernels of a split row hand on, per row: a record and four part sums for every 1024 tokens, the list's length and the list
+enum { SEGMENT = 1024, MAX_SEGMENTS = MAX_VOCAB / SEGMENT, RUNGS = 7 };
+struct Record { float max, z, rung[RUNGS], unused[7]; };         // the largest logit, the sum of exponentials against it; rungs: see k_sample_segments
+static_assert(sizeof(Record) == 64, "a record is four 16-byte words");
+static __host__ __device__ __forceinline__ uint64_t row_work(uint32_t vocab) { return (uint64_t)((vocab + SEGMENT - 1) / SEGMENT) * (sizeof(Record) + 32) + 64 + 8 * LIST; }
+struct RowWork {
+    Record *record;
+    uint64_t *part, *list;
+    uint32_t *count;
+    __device__ __forceinline__ RowWork(const SampleArgs &a, uint32_t row)
+    {
+        const uint32_t n = (a.vocab + SEGMENT - 1) / SEGMENT;
+        char *p = a.work + row * row_work(a.vocab);
+        record = (Record *)p;
+        part = (uint64_t *)(p + n * sizeof(Record));
+        count = (uint32_t *)(part + 4 * n);
+        list = (uint64_t *)((char *)count + 64);
+    }
 };
 
 // monotone in x; +0 and -0 alike
@@ -147,42 +168,41 @@ static __device__ __forceinline__ uint64_t sort_wave(uint64_t v, uint32_t lane)
     return v;
 }
 
-// One workgroup per row.  The row is read for the maxima, then once more (from the caches): for the sum of exponentials, the weights where a nucleus needs
-// their total, and a list of the largest tokens -- those that reach the k-th largest (top-k) or the 768th largest (a nucleus) of the threads' own
-// maxima.  Where the list holds what the filters leave, everything else happens on it; otherwise the filters read the row again.
+// A row of logits in stripes of 4096: thread t = 0 .. 1023 of stripe i has the four from 4096 i + 4 t
 template <typename T, bool BITS>
-__global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
-{
-    __shared__ Shared s;
-    const float NINF = -__builtin_huge_valf();
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, V = a.vocab;
-    const T *x = (const T *)a.logits + (uint64_t)row * a.row_stride;
-    const uint32_t *bits = BITS ? a.bits + (uint64_t)row * a.bits_stride : nullptr;
-    const uint32_t stripes = (V + STRIPE - 1) / STRIPE;
-    // Four logits of stripe i as they lie in memory, without a branch: lanes that reach over the end of the row read its last four (a row of less
-    // than four its first, again and again), and `unpack` moves them into place -- so that several stripes' loads are in flight at once
+struct Row {
+    // Four logits as they lie in memory, without a branch: lanes that reach over the end of the row read its last four (a row of less than four its
+    // first, again and again), and `unpack` moves them into place -- so that several stripes' loads are in flight at once
     typedef typename std::conditional<std::is_same<T, float>::value, f32x4, u32x2>::type Raw;
-    auto load = [&](uint32_t i, uint32_t t) -> Raw {
+    const T *x;
+    const uint32_t *bits;
+    uint32_t V;
+    __device__ __forceinline__ Row(const SampleArgs &a, uint32_t row)
+        : x((const T *)a.logits + (uint64_t)row * a.row_stride), bits(BITS ? a.bits + (uint64_t)row * a.bits_stride : nullptr), V(a.vocab) {}
+    __device__ __forceinline__ Raw load(uint32_t i, uint32_t t) const
+    {
         const uint32_t at = min(i * STRIPE + 4 * t, V < 4 ? 0 : V - 4);
         if constexpr (std::is_same<T, float>::value) {
             if (V >= 4) { const f32x4_a4 w = *(const f32x4_a4 *)(x + at); return f32x4{w[0], w[1], w[2], w[3]}; }
-            return f32x4{x[0], x[min(1u, V - 1)], x[min(2u, V - 1)], NINF};
+            return f32x4{x[0], x[min(1u, V - 1)], x[min(2u, V - 1)], -__builtin_huge_valf()};
         } else {
             const uint16_t *h = (const uint16_t *)x;
             if (V >= 4) { const u16x4_a2 w = *(const u16x4_a2 *)(h + at); return __builtin_bit_cast(u32x2, w); }
             return u32x2{(uint32_t)h[0] | ((uint32_t)h[min(1u, V - 1)] << 16), (uint32_t)h[min(2u, V - 1)]};
         }
-    };
-    auto load_bits = [&](uint32_t i, uint32_t t) -> uint32_t { return BITS ? bits[min(i * STRIPE + 4 * t, V - 1) >> 5] : 0; };
+    }
+    __device__ __forceinline__ uint32_t load_bits(uint32_t i, uint32_t t) const { return BITS ? bits[min(i * STRIPE + 4 * t, V - 1) >> 5] : 0; }
     // the logits as they are (-inf beyond the row); returns which of them may be drawn
-    auto unpack = [&](uint32_t i, uint32_t t, Raw w, uint32_t word, float v[4]) -> uint32_t {
+    __device__ __forceinline__ uint32_t unpack(uint32_t i, uint32_t t, Raw w, uint32_t word, float v[4]) const
+    {
+        const float NINF = -__builtin_huge_valf();
         const uint32_t at = i * STRIPE + 4 * t;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             if constexpr (std::is_same<T, float>::value) v[e] = w[e];
             else v[e] = as_f32(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
         }
-        if (i == stripes - 1) {
+        if ((i + 1) * STRIPE >= V) {
             if (V >= 4 && at + 4 > V) {
                 const uint32_t skip = at + 4 - V;
                 v[0] = skip == 1 ? v[1] : skip == 2 ? v[2] : skip == 3 ? v[3] : NINF;
@@ -196,59 +216,273 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
             }
         }
         return BITS ? (word >> (at & 31)) & 15u : 15u;
-    };
+    }
+};
+
+// A row's settings
+struct Settings {
+    float temperature, top_p, min_p;
+    int32_t top_k;
+    bool has_k, has_p;
+    __device__ __forceinline__ Settings(const SampleArgs &a, uint32_t row)
+    {
+        temperature = a.temperature_v ? a.temperature_v[row] : a.temperature;
+        top_k = a.top_k_v ? a.top_k_v[row] : a.top_k;
+        top_p = a.top_p_v ? a.top_p_v[row] : a.top_p;
+        min_p = a.min_p_v ? a.min_p_v[row] : a.min_p;
+        min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
+        if (!(temperature > 0.f)) { temperature = 1.f; top_k = 1; }                   // greedy: the first of the largest
+        has_k = top_k > 0 && (uint32_t)top_k < a.vocab;
+        has_p = top_p < 1.f;
+    }
+    // a list of the largest tokens is made for a nucleus of all, and where the k largest fit it
+    __device__ __forceinline__ bool lists() const { return has_k ? (uint32_t)top_k <= THREADS / 2 : has_p; }
+};
+
+// How a row's logits become weights and buckets; mz: the largest that may be drawn
+struct Scale {
+    double m, inv, floor_w;
+    float mz, c, low;
+    __device__ __forceinline__ Scale(const Settings &t, float mz_) : mz(mz_)
+    {
+        m = (double)mz;
+        inv = 1.4426950408889634074 / (double)t.temperature;
+        // buckets of 1 / 64 of a temperature below the largest logit: they order as the logits do (a rounded difference and product are monotone)
+        c = fminf(64.f / t.temperature, 1e30f);
+        // a logit below `low` has no weight: less than min_p of the largest, or 2^-45
+        floor_w = t.min_p > 0.f ? (double)t.min_p * 17592186044416.0 : 0.0;
+        const float reach = mz - t.temperature * fminf(31.5f, t.min_p > 0.f ? 1e-3f - 0.69314718f * __builtin_amdgcn_logf(t.min_p) : 31.5f) * 1.00001f;
+        low = fmaxf(reach, -3.402823466e38f);
+    }
+    __device__ __forceinline__ uint32_t bucket(float v) const { const float b = (mz - v) * c; return b < (float)(BUCKETS - 1) ? (uint32_t)b : (uint32_t)(BUCKETS - 1); }
+};
+
+// The first kernel of a split row, a wave for every 1024 tokens: their largest logit and sum of exponentials, and rungs -- of the lanes' own maxima (16 tokens that may
+// be drawn) the largest, 2nd, 4th, 8th, 16th, 32nd and 56th.  The rungs of all waves tell a logit that at least so and so many tokens reach.
+static __device__ __forceinline__ uint32_t rung_rank(uint32_t i) { return i < 6 ? 1u << i : 56u; }
+template <typename T, bool BITS>
+__global__ __launch_bounds__(256) void k_sample_segments(SampleArgs a)
+{
+    const float NINF = -__builtin_huge_valf(), L2E = 1.4426950408889634f;
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), seg = blockIdx.x * 4 + wave, row = blockIdx.y;
+    if (seg * SEGMENT >= a.vocab) return;
+    const Row<T, BITS> x(a, row);
+    RowWork out(a, row);
+    typename Row<T, BITS>::Raw w[4];
+    uint32_t b[4];
+    float v[4][4], mx = NINF, mz = NINF;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) { w[j] = x.load(blockIdx.x, wave * 256 + j * 64 + lane); b[j] = x.load_bits(blockIdx.x, wave * 256 + j * 64 + lane); }
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+        const uint32_t ok = x.unpack(blockIdx.x, wave * 256 + j * 64 + lane, w[j], b[j], v[j]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[j][e] = clean(v[j][e]);
+            mx = fmaxf(mx, v[j][e]);
+            if (BITS) mz = fmaxf(mz, (ok >> e) & 1 ? v[j][e] : NINF);
+        }
+    }
+    const float own = BITS ? mz : mx;
+    mx = wave_max(mx);
+    float z = 0.f;
+    if (mx > NINF) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) z += __builtin_amdgcn_exp2f((v[j][e] - mx) * L2E);
+    }
+    for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o);
+    uint32_t above = 0, reach = 0;                               // lanes with a larger maximum, with one at least as large
+#pragma unroll
+    for (int l = 0; l < 64; l++) {
+        const float o = as_f32((uint32_t)__builtin_amdgcn_readlane((int)as_u32(own), l));
+        above += o > own;
+        reach += o >= own;
+    }
+    Record &r = out.record[seg];
+#pragma unroll
+    for (uint32_t i = 0; i < RUNGS; i++) if (above < rung_rank(i) && rung_rank(i) <= reach) r.rung[i] = own;    // (equal lanes write the same)
+    if (lane == 0) { r.max = mx; r.z = z; if (seg == 0) *out.count = 0; }
+}
+
+// The largest logit of a row and the largest that may be drawn, from its records (every thread below `segments` has read its own)
+static __device__ __forceinline__ void row_maxima(const Record &r, float *shared, uint32_t lane, uint32_t wave, float &mx, float &mz)
+{
+    mx = wave_max(r.max);
+    mz = wave_max(r.rung[0]);
+    if (lane == 0 && wave < 4) { shared[wave] = mx; shared[4 + wave] = mz; }
+    __syncthreads();
+    mx = wave_max(shared[lane & 3]);
+    mz = wave_max(shared[4 + (lane & 3)]);
+}
+static __device__ __forceinline__ Record no_record()
+{
+    Record r;
+    r.max = -__builtin_huge_valf();
+    r.z = 0.f;
+#pragma unroll
+    for (int i = 0; i < RUNGS; i++) r.rung[i] = -__builtin_huge_valf();
+    return r;
+}
+
+// The second: the row's tokens in buckets as high as its rungs ask for go on its list, and the weights of every 256 tokens are added up (those of min_p where no other filter
+// is on; not at all under a top_k, which weighs no more than its list).
+template <typename T, bool BITS>
+__global__ __launch_bounds__(256) void k_sample_lists(SampleArgs a)
+{
+    __shared__ uint32_t s_count[BUCKETS], s_wave[4], s_bucket;
+    __shared__ float s_max[8];
+    __shared__ double s_root[32];
+    const float NINF = -__builtin_huge_valf(), LOWEST = -3.402823466e38f;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), row = blockIdx.y, seg = blockIdx.x * 4 + wave;
+    const uint32_t segments = (a.vocab + SEGMENT - 1) / SEGMENT;
+    const Row<T, BITS> x(a, row);
+    RowWork out(a, row);
+    typename Row<T, BITS>::Raw w[4];
+    uint32_t b[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) { w[j] = x.load(blockIdx.x, wave * 256 + j * 64 + lane); b[j] = x.load_bits(blockIdx.x, wave * 256 + j * 64 + lane); }
+    Record r = tid < segments ? out.record[tid] : no_record();
+    const Settings t(a, row);
+    if (tid < 32) s_root[tid] = exp2((double)tid / 32.0);
+    float mx, mz;
+    row_maxima(r, s_max, lane, wave, mx, mz);
+    if (mz == NINF) return;
+    const Scale sc(t, mz);
+    uint32_t last = 0;                                           // tokens of this bucket and those before go on the list
+    if (t.lists()) {
+        const uint32_t want = t.has_k ? (uint32_t)t.top_k : min(900u, 32 * segments);
+#pragma unroll
+        for (uint32_t i = 0; i < BUCKETS / 256; i++) s_count[i * 256 + tid] = 0;
+        if (tid == 0) s_bucket = BUCKETS - 1;                    // (not so many: all of them)
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < RUNGS; i++) if (r.rung[i] > NINF) atomicAdd(&s_count[sc.bucket(r.rung[i])], rung_rank(i) - (i ? rung_rank(i - 1) : 0));
+        __syncthreads();
+        uint32_t mine[8], sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) { mine[i] = s_count[tid * 8 + i]; sum += mine[i]; }
+        uint32_t incl = (uint32_t)wave_scan(sum);
+        if (lane == 63) s_wave[wave] = incl;
+        __syncthreads();
+        for (uint32_t o = 0; o < wave; o++) incl += s_wave[o];
+        uint32_t run = incl - sum;
+        if (run < want && incl >= want) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) { if (run < want && run + mine[i] >= want) s_bucket = tid * 8 + i; run += mine[i]; }
+        }
+        __syncthreads();
+        last = s_bucket;
+    }
+    if (seg >= segments) return;
+    uint64_t entry[16];
+    uint32_t n = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+        const uint32_t st = wave * 256 + j * 64 + lane, at = blockIdx.x * STRIPE + 4 * st;
+        float v[4];
+        const uint32_t ok = x.unpack(blockIdx.x, st, w[j], b[j], v);
+        double mass = 0.0;                                       // (whole numbers below 2^53: exact)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            v[e] = clean(v[e]);
+            const bool may = v[e] >= LOWEST && (!BITS || ((ok >> e) & 1));
+            if (may && !t.has_k && (t.has_p || v[e] >= sc.low)) {
+                const double we = weight(v[e], sc.m, sc.inv, s_root);
+                if (t.has_p || we >= sc.floor_w) mass += we;
+            }
+            entry[4 * j + e] = may && t.lists() && sc.bucket(v[e]) <= last ? ((uint64_t)key_of(v[e]) << 32) | (uint32_t)~(at + e) : 0;
+            n += entry[4 * j + e] != 0;
+        }
+        if (!t.has_k) {
+            const uint64_t sum = wave_scan((uint64_t)mass);
+            if (lane == 63) out.part[seg * 4 + j] = sum;
+        }
+    }
+    if (!t.lists()) return;
+    const uint32_t incl = (uint32_t)wave_scan(n), all = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+    if (!all) return;
+    uint32_t at = 0;
+    if (lane == 0) at = __hip_atomic_fetch_add(out.count, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + incl - n;
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        if (entry[i]) { if (at < LIST) out.list[at] = entry[i]; at++; }
+}
+
+// One workgroup per row.  The row is read for the maxima, then once more (from the caches): for the sum of exponentials, the weights where a nucleus needs
+// their total, and a list of the largest tokens -- those that reach the k-th largest (top-k) or the 768th largest (a nucleus) of the threads' own
+// maxima.  Where the list holds what the filters leave, everything else happens on it; otherwise the filters read the row again.
+template <typename T, bool BITS, bool SPLIT>
+__global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(SampleArgs a)
+{
+    __shared__ Shared s;
+    const float NINF = -__builtin_huge_valf();
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, V = a.vocab;
+    const Row<T, BITS> x(a, row);
+    typedef typename Row<T, BITS>::Raw Raw;
+    const uint32_t stripes = (V + STRIPE - 1) / STRIPE;
     auto row_pass = [&](auto f) {                                // f(index of the first, four logits, which may be drawn)
         enum { FLY = 4 };
         for (uint32_t i0 = 0; i0 < stripes; i0 += FLY) {
             Raw w[FLY];
             uint32_t b[FLY];
 #pragma unroll
-            for (uint32_t j = 0; j < FLY; j++) { const uint32_t i = min(i0 + j, stripes - 1); w[j] = load(i, tid); b[j] = load_bits(i, tid); }
+            for (uint32_t j = 0; j < FLY; j++) { const uint32_t i = min(i0 + j, stripes - 1); w[j] = x.load(i, tid); b[j] = x.load_bits(i, tid); }
 #pragma unroll
             for (uint32_t j = 0; j < FLY; j++)
-                if (i0 + j < stripes) { float v[4]; const uint32_t ok = unpack(i0 + j, tid, w[j], b[j], v); f((i0 + j) * STRIPE + 4 * tid, v, ok); }
+                if (i0 + j < stripes) { float v[4]; const uint32_t ok = x.unpack(i0 + j, tid, w[j], b[j], v); f((i0 + j) * STRIPE + 4 * tid, v, ok); }
         }
     };
     if (tid < 32) s.root[tid] = exp2((double)tid / 32.0);
     // the largest logit, and the largest that may be drawn (fmaxf leaves NaN out)
     const float L2E = 1.4426950408889634f;
-    float mx = NINF, mz = NINF;
-    row_pass([&](uint32_t, const float *v, uint32_t ok) {
+    float mx = NINF, mz = NINF, own = NINF;                      // own: the thread's largest that may be drawn
+    Record rec;
+    uint64_t part = 0;
+    uint32_t on_list = 0;
+    if constexpr (SPLIT) {
+        const uint32_t segments = (V + SEGMENT - 1) / SEGMENT;
+        const RowWork in(a, row);
+        rec = tid < segments ? in.record[tid] : no_record();
+        part = tid < 4 * segments ? in.part[tid] : 0;
+        on_list = *in.count;
+        s.list[tid] = in.list[tid];                              // (all of it: its length is on its way, too)
+        s.list[tid + THREADS] = in.list[tid + THREADS];
+        row_maxima(rec, s.wavef, lane, wave, mx, mz);
+    } else {
+        row_pass([&](uint32_t, const float *v, uint32_t ok) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            mx = fmaxf(mx, v[e]);
-            if (BITS) mz = fmaxf(mz, (ok >> e) & 1 ? v[e] : NINF);
-        }
-    });
-    const float own = clean(BITS ? mz : mx);                     // the thread's own
-    mx = wave_max(mx);
-    mz = BITS ? wave_max(mz) : mx;
-    if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; }
-    __syncthreads();
-    mx = clean(wave_max(s.wavef[lane % WAVES]));
-    mz = clean(wave_max(s.wavef[WAVES + lane % WAVES]));
+            for (int e = 0; e < 4; e++) {
+                mx = fmaxf(mx, v[e]);
+                if (BITS) mz = fmaxf(mz, (ok >> e) & 1 ? v[e] : NINF);
+            }
+        });
+        own = clean(BITS ? mz : mx);
+        mx = wave_max(mx);
+        mz = BITS ? wave_max(mz) : mx;
+        if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; }
+        __syncthreads();
+        mx = clean(wave_max(s.wavef[lane % WAVES]));
+        mz = clean(wave_max(s.wavef[WAVES + lane % WAVES]));
+    }
     if (mz == NINF) {                                            // nothing may be drawn
         for (uint32_t d = tid; d < a.draws; d += THREADS) { a.tokens[(uint64_t)row * a.draws + d] = -1; a.logprobs[(uint64_t)row * a.draws + d] = NINF; }
         return;
     }
-    float temperature = a.temperature_v ? a.temperature_v[row] : a.temperature;
-    int32_t top_k = a.top_k_v ? a.top_k_v[row] : a.top_k;
-    const float top_p = a.top_p_v ? a.top_p_v[row] : a.top_p;
-    float min_p = a.min_p_v ? a.min_p_v[row] : a.min_p;
-    min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
-    if (!(temperature > 0.f)) { temperature = 1.f; top_k = 1; }                       // greedy: the first of the largest
-    const double inv = 1.4426950408889634074 / (double)temperature, m = (double)mz;
-    auto weigh = [&](float v) { return weight(v, m, inv, s.root); };
+    const Settings set(a, row);
+    const Scale sc(set, mz);
+    auto weigh = [&](float v) { return weight(v, sc.m, sc.inv, s.root); };
     auto one = [](float) { return 1.0; };
-    // buckets of 1 / 64 of a temperature below the largest logit: they order as the logits do (a rounded difference and product are monotone)
-    const float c = fminf(64.f / temperature, 1e30f);
-    auto bucket0 = [&](float v) { const float b = (mz - v) * c; return b < (float)(BUCKETS - 1) ? (uint32_t)b : (uint32_t)(BUCKETS - 1); };
+    auto bucket0 = [&](float v) { return sc.bucket(v); };
     auto value_of = [](uint64_t e) { const uint32_t k = (uint32_t)(e >> 32); return as_f32((k >> 31) ? k ^ 0x80000000u : ~k); };
     uint32_t thr = 0, lim = 0xffffffffu;                         // kept: key > thr, or key == thr and index <= lim
     auto kept = [&](float v, uint32_t idx) { const uint32_t k = key_of(v); return k > thr || (k == thr && idx <= lim); };
     // The sum of exponentials over the whole row (fp32: it enters the log-probabilities only), added up by the first pass behind the maxima; v cleaned
     float z = 0.f;
-    bool have_z = false;
+    bool have_z = SPLIT;
+    if (SPLIT && rec.max > NINF) z = rec.z * __builtin_amdgcn_exp2f((rec.max - mx) * L2E);
     auto add_z = [&](const float *v) {
 #pragma unroll
         for (int e = 0; e < 4; e++) z += __builtin_amdgcn_exp2f((v[e] - mx) * L2E);
@@ -376,7 +610,7 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
         if (at != 0xffffffffu && wave == 0) {                   // those 256 logits again, in order
             float v[4];
             const uint32_t i = at / WAVES, t = (at % WAVES) * 64 + lane, idx = at * 256 + 4 * lane;
-            uint32_t ok = unpack(i, t, load(i, t), load_bits(i, t), v), mine = 0;
+            uint32_t ok = x.unpack(i, t, x.load(i, t), x.load_bits(i, t), v), mine = 0;
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) { if (!(clean(v[e]) >= LOWEST) || key_of(clean(v[e])) != thr || idx + e > old_lim) ok &= ~(1u << e); mine += (ok >> e) & 1; }
             const uint32_t rank = (uint32_t)wave_scan(mine) - mine, want = (uint32_t)(stay - s.before);
@@ -397,12 +631,16 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
         row_from(LOWEST, f, [&](const float *v, uint32_t) { if (with_z) add_z(v); });
     };
 
-    const bool has_k = top_k > 0 && (uint32_t)top_k < V, has_p = top_p < 1.f;
-    const uint64_t k = (uint64_t)top_k;
-    const double p = (double)fmaxf(top_p, 0.f);
+    const bool has_k = set.has_k, has_p = set.has_p;
+    const uint64_t k = (uint64_t)set.top_k;
+    const double p = (double)fmaxf(set.top_p, 0.f);
     double own_mass = 0.0;                                       // (whole numbers below 2^53: exact)
     uint64_t total = 0;                                          // the weight that a nucleus is a part of
-    if ((has_k && k <= THREADS / 2) || (has_p && !has_k)) {
+    if (SPLIT) {
+        if (set.lists() && on_list <= LIST) listed = on_list;
+        if (!has_k) block_scan(part, s, lane, wave, total);
+        __syncthreads();
+    } else if (set.lists()) {
         // the smallest of the `want` largest of the threads' maxima: at least `want` tokens reach it
         const uint64_t want = has_k ? k : 3 * THREADS / 4;
         clear_buckets();
@@ -474,10 +712,9 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
             shorten(row_all, weigh, reached);
         }
     }
-    // The weights of what is left, summed for every 256 tokens (a logit below `reach` has none: less than min_p of the largest weight, or 2^-45)
-    const double floor_w = min_p > 0.f ? (double)min_p * 17592186044416.0 : 0.0;
-    const float reach = mz - temperature * fminf(31.5f, min_p > 0.f ? 1e-3f - 0.69314718f * __builtin_amdgcn_logf(min_p) : 31.5f) * 1.00001f;
-    const float low = fmaxf(reach, LOWEST);
+    // The weights of what is left, summed for every 256 tokens
+    const double floor_w = sc.floor_w;
+    const float low = sc.low;
     auto final_weight = [&](float v, uint32_t idx) -> uint64_t {
         if (!(v >= low) || !kept(v, idx)) return 0;
         const double w = weigh(v);
@@ -485,9 +722,10 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
     };
     const uint32_t parts = stripes * WAVES;
     __syncthreads();
-    s.part[tid] = 0;
+    s.part[tid] = SPLIT && !has_k && !has_p ? part : 0;
     __syncthreads();
-    if (listed) list_pass([&](float v, uint32_t idx) { const uint64_t w = final_weight(v, idx); if (w) atomicAdd((unsigned long long *)&s.part[idx >> 8], (unsigned long long)w); });
+    if (SPLIT && !has_k && !has_p) {}
+    else if (listed) list_pass([&](float v, uint32_t idx) { const uint64_t w = final_weight(v, idx); if (w) atomicAdd((unsigned long long *)&s.part[idx >> 8], (unsigned long long)w); });
     else
         row_pass([&](uint32_t at, float *v, uint32_t ok) {
             uint64_t w = 0;
@@ -512,6 +750,7 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
     for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o);
     if (lane == 0) s.wavef[wave] = z;
     __syncthreads();
+    if (wave >= a.draws) return;
     double lse = 0.0;
     for (int w = 0; w < WAVES; w++) lse += (double)s.wavef[w];
     lse = (double)mx + log(lse);
@@ -527,7 +766,7 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
         float v[4];
         uint64_t w[4];
         const uint32_t i = lo / WAVES, t = (lo % WAVES) * 64 + lane, idx = lo * 256 + 4 * lane;
-        const uint32_t ok = unpack(i, t, load(i, t), load_bits(i, t), v);
+        const uint32_t ok = x.unpack(i, t, x.load(i, t), x.load_bits(i, t), v);
 #pragma unroll
         for (uint32_t e = 0; e < 4; e++) { v[e] = clean(v[e]); w[e] = !BITS || ((ok >> e) & 1) ? final_weight(v[e], idx + e) : 0; }
         const uint64_t mine = w[0] + w[1] + w[2] + w[3], sum = wave_scan(mine);
@@ -548,34 +787,50 @@ __global__ __launch_bounds__(THREADS, 8) void k_sample_tokens(SampleArgs a)
 }
 
 template <typename T>
-static int sample_tokens(void *stream, const SampleArgs &a)
+static int sample_tokens(void *stream, const SampleArgs &a, uint64_t work_bytes)
 {
     if (!a.rows || !a.draws) return FMI_OK;
     if (!a.vocab || a.vocab > MAX_VOCAB) { fmi_set_error("sealnn_sample_tokens: a vocabulary of %u (1 .. %u)", a.vocab, (unsigned)MAX_VOCAB); return FMI_ERR_UNSUPPORTED; }
     if (!a.logits || !a.u || !a.tokens || !a.logprobs || ((uintptr_t)a.logits & (sizeof(T) - 1))) { fmi_set_error("sealnn_sample_tokens: null or misaligned argument"); return FMI_ERR_ARG; }
-    if (a.bits) hipLaunchKernelGGL((k_sample_tokens<T, true>), dim3(a.rows), dim3(THREADS), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((k_sample_tokens<T, false>), dim3(a.rows), dim3(THREADS), 0, (hipStream_t)stream, a);
+    if (a.work && (a.vocab < 4 || a.rows > 65535 || work_bytes < a.rows * row_work(a.vocab) || ((uintptr_t)a.work & 15))) {
+        fmi_set_error("sealnn_sample_tokens: %u rows of %u in a workspace of %llu bytes (16-byte aligned; %llu for a row of at least 4, at most 65535 rows)", a.rows, a.vocab,
+                      (unsigned long long)work_bytes, (unsigned long long)row_work(a.vocab));
+        return FMI_ERR_ARG;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    auto go = [&](auto bits) {
+        constexpr bool B = decltype(bits)::value;
+        if (!a.work) { hipLaunchKernelGGL((k_sample_tokens<T, B, false>), dim3(a.rows), dim3(THREADS), 0, st, a); return; }
+        const dim3 grid((a.vocab + STRIPE - 1) / STRIPE, a.rows);
+        hipLaunchKernelGGL((k_sample_segments<T, B>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_sample_lists<T, B>), grid, dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_sample_tokens<T, B, true>), dim3(a.rows), dim3(THREADS), 0, st, a);
+    };
+    if (a.bits) go(std::true_type());
+    else go(std::false_type());
     NNCHK();
     return FMI_OK;
 }
 
 static SampleArgs sample_args(const void *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float *u, uint32_t draws, const uint32_t *bits,
                               uint64_t bits_stride, float temperature, int32_t top_k, float top_p, float min_p, const float *temperature_v,
-                              const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs)
+                              const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs, void *work)
 {
     SampleArgs a;
     a.logits = logits; a.row_stride = row_stride; a.bits = bits; a.bits_stride = bits_stride; a.u = u;
     a.temperature_v = temperature_v; a.top_p_v = top_p_v; a.min_p_v = min_p_v; a.top_k_v = top_k_v;
     a.rows = rows; a.vocab = vocab; a.draws = draws; a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
-    a.tokens = tokens; a.logprobs = logprobs;
+    a.tokens = tokens; a.logprobs = logprobs; a.work = (char *)work;
     return a;
 }
 
 extern "C" int sealnn_sample_tokens(void *stream, const float *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float *u, uint32_t draws,
                                     const uint32_t *bits, uint64_t bits_stride, float temperature, int32_t top_k, float top_p, float min_p,
-                                    const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs)
-{ return sample_tokens<float>(stream, sample_args(logits, row_stride, rows, vocab, u, draws, bits, bits_stride, temperature, top_k, top_p, min_p, temperature_v, top_k_v, top_p_v, min_p_v, tokens, logprobs)); }
+                                    const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs,
+                                    void *work, uint64_t work_bytes)
+{ return sample_tokens<float>(stream, sample_args(logits, row_stride, rows, vocab, u, draws, bits, bits_stride, temperature, top_k, top_p, min_p, temperature_v, top_k_v, top_p_v, min_p_v, tokens, logprobs, work), work_bytes); }
 extern "C" int sealnn_sample_tokens_bf16(void *stream, const void *logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float *u, uint32_t draws,
                                          const uint32_t *bits, uint64_t bits_stride, float temperature, int32_t top_k, float top_p, float min_p,
-                                         const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs)
-{ return sample_tokens<bf16>(stream, sample_args(logits, row_stride, rows, vocab, u, draws, bits, bits_stride, temperature, top_k, top_p, min_p, temperature_v, top_k_v, top_p_v, min_p_v, tokens, logprobs)); }
+                                         const float *temperature_v, const int32_t *top_k_v, const float *top_p_v, const float *min_p_v, int64_t *tokens, float *logprobs,
+                                         void *work, uint64_t work_bytes)
+{ return sample_tokens<bf16>(stream, sample_args(logits, row_stride, rows, vocab, u, draws, bits, bits_stride, temperature, top_k, top_p, min_p, temperature_v, top_k_v, top_p_v, min_p_v, tokens, logprobs, work), work_bytes); }

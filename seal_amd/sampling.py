@@ -1,7 +1,7 @@
 """Drawing tokens from logits on the GPU: temperature, top-k, top-p and min-p, under an optional allowed-token bitmap (the FM-index
 constraint of a step, ``IndexBasedLogitsProcessor.allowed_bits``), from random numbers that the caller gives.
 
-``sample_tokens`` is one kernel launch (``sealnn_sample_tokens``, include/sealnn.h); ``fm_index_sample`` (beam_search.py) is the decode loop
+``sample_tokens`` calls the library once (``sealnn_sample_tokens``, include/sealnn.h: one kernel, or three for few rows of a large vocabulary); ``fm_index_sample`` (beam_search.py) is the decode loop
 around it.  The reference draws with ``torch.multinomial`` over the softmax (reference beam_search.py:296, ``sample=True``)."""
 from typing import Optional, Tuple, Union
 
@@ -10,6 +10,9 @@ import torch
 from ._lib import launch, lib
 
 MAX_VOCAB = 1 << 18
+# Few rows of a large vocabulary are spread over the card by three kernels instead of one workgroup each (include/sealnn.h).  us, one kernel / three, fp32, top-p 0.9: 1 x 16384
+# 22.7 / 23.5, 1 x 50265 36.7 / 24.4, 32 x 50265 38 / 28, 128 x 50265 40.5 / 41.8, 1 x 131072 60.7 / 25.0; top-k 50: 1 x 50265 19.2 / 20.5, 64 x 50265 21.4 / 26.5, 1 x 131072 26.1 / 20.4
+SPLIT_VOCAB, SPLIT_ROWS = 32768, 32
 Setting = Union[float, int, torch.Tensor]
 
 
@@ -85,6 +88,11 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     if not logits.is_cuda:
         raise RuntimeError("sample_tokens: the logits must live on the GPU (seal_amd has no CPU path)")
     tokens, logprobs = u.new_empty(u_shape, dtype=torch.int64), u.new_empty(u_shape)
+    work, work_bytes = None, 0
+    if vocab >= SPLIT_VOCAB and rows <= SPLIT_ROWS:
+        work_bytes = rows * (-(-vocab // 1024) * 96 + 16448)
+        work = torch.empty(work_bytes, dtype=torch.uint8, device=dev)
     launch(lib().sealnn_sample_tokens if dt == torch.float32 else lib().sealnn_sample_tokens_bf16, logits.get_device(), logits.data_ptr(), row_stride, rows, vocab,
-           u.data_ptr(), u_shape[1] if len(u_shape) == 2 else 1, bits, bits_stride, t, k, p, m, t_v, k_v, p_v, m_v, tokens.data_ptr(), logprobs.data_ptr())
+           u.data_ptr(), u_shape[1] if len(u_shape) == 2 else 1, bits, bits_stride, t, k, p, m, t_v, k_v, p_v, m_v, tokens.data_ptr(), logprobs.data_ptr(),
+           None if work is None else work.data_ptr(), work_bytes)
     return tokens, logprobs

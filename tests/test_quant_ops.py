@@ -147,9 +147,13 @@ def test_c_entries_refuse_before_they_launch():
                lambda: at(None, None, 64, 64, p, p, p, p, p, None, 0, 1, 1, 1, 1, 64, 16, 64, 1.0, 1, None, 0, p),
                lambda: at(None, p, 64, 64, p, p, p, p, p, None, 0, 1, 1, 1, 1, 64, 16, 96, 1.0, 1, None, 0, p),
                lambda: at(None, p, 64, 64, p, p, p, p, p, None, 0, 1 << 20, 1 << 10, 64, 1, 64, 16, 64, 1.0, 1, None, 0, p),
-               lambda: sm(None, p, 10, 1, (1 << 18) + 1, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p),
-               lambda: sm(None, p, 10, 1, 0, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p),
-               lambda: sm(None, None, 10, 1, 10, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p)]
+               lambda: sm(None, p, 10, 1, (1 << 18) + 1, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, None, 0),
+               lambda: sm(None, p, 10, 1, 0, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, None, 0),
+               lambda: sm(None, None, 10, 1, 10, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, None, 0),
+               lambda: sm(None, p, 10, 1, 10, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, p, 96 + 16448 - 1),
+               lambda: sm(None, p, 10, 1, 10, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, p + 8, 1 << 20),
+               lambda: sm(None, p, 10, 65536, 10, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, p, 1 << 40),
+               lambda: sm(None, p, 10, 1, 3, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, p, 1 << 20)]
         for i, f in enumerate(bad):
             with pytest.raises(SealFMError) as e:
                 check(f())
@@ -158,4 +162,4 @@ def test_c_entries_refuse_before_they_launch():
         check(w4(None, p, 128, p, p, None, 0, 16, 128, 32, 0, p))
         check(ap(None, p, p, st, 0, p, None, p, p, p, p, 1, 1, 64, 16, 64))
         check(at(None, p, 64, 64, p, p, p, p, p, None, 0, 0, 1, 1, 1, 64, 16, 64, 1.0, 1, None, 0, p))
-        check(sm(None, p, 10, 0, 10, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p))
+        check(sm(None, p, 10, 0, 10, p, 1, None, 0, 1.0, 0, 1.0, 0.0, None, None, None, None, p, p, None, 0))
