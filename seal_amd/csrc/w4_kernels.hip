@@ -55,34 +55,127 @@ static __device__ __forceinline__ bf16x8 codes8(uint32_t w)
     return __builtin_bit_cast(bf16x8, o);
 }
 
-// A workgroup of eight waves: `kw` of them (1, 2, 4 or 8) take the 128-column chunks in turn, 8 / kw such teams have NT tiles of 16 outputs x MT tiles of 16 rows of x
-// each; a team's sums meet in LDS.  GS: matrix instructions per scale group (group / 32).  The planes of x are made once for the NT tiles.  Rows of x
-// beyond the last repeat it: what a matrix instruction makes of them is not stored.
-template <typename T, int NT, int MT, int GS>
-__global__ __launch_bounds__(512) void k_w4_linear(const T *x, uint64_t x_stride, const uint32_t *codes, const uint16_t *scales, const T *bias,
-                                                   uint32_t M, uint32_t N, uint32_t K, uint32_t kw, uint32_t vec, uint32_t gelu, T *y)
+// acc += scales * d: the scales of four outputs, bf16
+static __device__ __forceinline__ void add_scaled(f32x4 &acc, u32x2 sc, f32x4 d)
+{
+    const f32x4 f = {as_f32(sc[0] << 16), as_f32(sc[0] & 0xffff0000u), as_f32(sc[1] << 16), as_f32(sc[1] & 0xffff0000u)};
+#pragma unroll
+    for (int r = 0; r < 4; r++) acc[r] = fmaf(f[r], d[r], acc[r]);
+}
+
+// one output: bias, GELU, the only rounding to T
+template <typename T>
+static __device__ __forceinline__ void put(float v, const T *bias, uint32_t gelu, uint32_t row, uint32_t out, uint32_t N, T *y)
+{
+    if (out >= N) return;
+    v += bias ? load1(bias + out) : 0.f;
+    if (gelu) v = 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    store1(y + (uint64_t)row * N + out, v);
+}
+
+// More than 1024 columns: a workgroup of W waves has NT tiles of 16 outputs and 16 rows of x, the waves take the 128-column chunks in turn and their sums meet
+// in LDS.  GS: matrix instructions per scale group (group / 32).  Rows of x beyond the last repeat it: what a matrix instruction makes of them is not stored.
+template <typename T, int NT, int GS, int W>
+__global__ __launch_bounds__(64 * W) void k_w4_linear_long(const T *x, uint64_t x_stride, const uint32_t *codes, const uint16_t *scales, const T *bias,
+                                                           uint32_t M, uint32_t N, uint32_t K, uint32_t vec, uint32_t gelu, T *y)
 {
     enum { XP = XPlanes<T>::N, GROUPS = 4 / GS };
-    __shared__ f32x4 s_sum[8][NT][MT][64];
+    __shared__ f32x4 s_sum[W][NT][64];
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), col = lane & 15, g = lane >> 4;
-    const uint32_t tiles = (N + 15) / 16, chunks = (K + 127) / 128, team = wave / kw, part = wave % kw;
-    const uint32_t tile0 = (blockIdx.x * (8 / kw) + team) * NT, m0 = blockIdx.y * MT * 16;
-    f32x4 acc[NT][MT];
+    const uint32_t tiles = (N + 15) / 16, chunks = (K + 127) / 128, tile0 = blockIdx.x * NT, row = blockIdx.y * 16 + col;
+    const T *xr = x + (uint64_t)min(row, M - 1) * x_stride;
+    f32x4 acc[NT];
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int n = 0; n < NT; n++) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t c = wave; c < chunks; c += W) {
+        u32x4 w[NT];
+        u32x2 sc[NT][GROUPS];
 #pragma unroll
-        for (int m = 0; m < MT; m++) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (tile0 < tiles)
-        for (uint32_t c = part; c < chunks; c += kw) {
-            u32x4 w[NT];
-            u32x2 sc[NT][GROUPS];
+        for (int n = 0; n < NT; n++) {
+            const uint64_t t = min(tile0 + n, tiles - 1);           // (a tile beyond the last reads the last and is not stored)
+            w[n] = *(const u32x4 *)(codes + (t * chunks + c) * 256 + lane * 4);
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const uint64_t t = min(tile0 + n, tiles - 1);           // (a tile beyond the last reads the last and is not stored)
-                w[n] = *(const u32x4 *)(codes + (t * chunks + c) * 256 + lane * 4);
+            for (int q = 0; q < GROUPS; q++) sc[n][q] = *(const u32x2 *)(scales + ((t * chunks + c) * GROUPS + q) * 16 + 4 * g);
+        }
 #pragma unroll
-                for (int q = 0; q < GROUPS; q++) sc[n][q] = *(const u32x2 *)(scales + ((t * chunks + c) * GROUPS + q) * 16 + 4 * g);
+        for (int q = 0; q < GROUPS; q++) {
+            f32x4 d[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) d[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = q * GS; s < (q + 1) * GS; s++) {
+                bf16x8 b[XP];
+                load_x<T>(xr, 128 * c + 32 * s + 8 * g, K, vec, b);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const bf16x8 a = codes8(w[n][s]);
+#pragma unroll
+                    for (int p = 0; p < XP; p++) d[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[p], d[n], 0, 0, 0);
+                }
             }
+#pragma unroll
+            for (int n = 0; n < NT; n++) add_scaled(acc[n], sc[n][q], d[n]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++) s_sum[wave][n][lane] = acc[n];
+    __syncthreads();
+    if (wave >= NT) return;
+    f32x4 v = s_sum[0][wave][lane];
+#pragma unroll
+    for (uint32_t o = 1; o < W; o++) v += s_sum[o][wave][lane];
+    if (row >= M) return;
+#pragma unroll
+    for (uint32_t r = 0; r < 4; r++) put(v[r], bias, gelu, row, (tile0 + wave) * 16 + 4 * g + r, N, y);
+}
+
+// At most 1024 columns: `kw` of a workgroup's eight waves (1, 2, 4 or 8) have one 128-column chunk each, 8 / kw such teams NT tiles of 16 outputs x MT tiles of 16 rows of
+// x.  A wave's chunk of x stays in its registers as planes (splitting fp32 into them costs more instructions than the products) while the workgroup goes
+// from tiles to tiles, every gridDim.x * 8 / kw * NT; the next round's codes are on their way while it works on these.  The waves' sums of two rounds lie side by side in LDS:
+// one barrier a round.  1 x 50265 x 1024 fp32 in 11.0 us, 2.5 TB/s of codes and scales; a launch and the first loads are 4 of them.
+template <typename T, int NT, int MT, int GS>
+__global__ __launch_bounds__(512, 2) void k_w4_linear_many(const T *x, uint64_t x_stride, const uint32_t *codes, const uint16_t *scales, const T *bias,
+                                                           uint32_t M, uint32_t N, uint32_t K, uint32_t kw, uint32_t vec, uint32_t gelu, T *y)
+{
+    enum { XP = XPlanes<T>::N, GROUPS = 4 / GS };
+    __shared__ f32x4 s_sum[2][8][NT][MT][64];
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), col = lane & 15, g = lane >> 4;
+    const uint32_t tiles = (N + 15) / 16, chunks = (K + 127) / 128, teams = 8 / kw, team = wave / kw, c = wave % kw, m0 = blockIdx.y * MT * 16;
+    const uint32_t step = gridDim.x * teams * NT, first = blockIdx.x * teams * NT, mine = first + team * NT;
+    const bool has = c < chunks;                                 // (kw waves, maybe fewer chunks)
+    const uint32_t cc = has ? c : 0;
+    u32x4 w[NT];
+    u32x2 sc[NT][GROUPS];
+    auto fetch = [&](uint32_t tile0) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const uint64_t t = min(tile0 + n, tiles - 1);           // (a tile beyond the last reads the last and is not stored)
+            w[n] = *(const u32x4 *)(codes + (t * chunks + cc) * 256 + lane * 4);
+#pragma unroll
+            for (int q = 0; q < GROUPS; q++) sc[n][q] = *(const u32x2 *)(scales + ((t * chunks + cc) * GROUPS + q) * 16 + 4 * g);
+        }
+    };
+    fetch(mine);
+    bf16x8 b[4][MT][XP];
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) load_x<T>(x + (uint64_t)min(m0 + 16 * m + col, M - 1) * x_stride, 128 * cc + 32 * s + 8 * g, K, vec, b[s][m]);
+    uint32_t side = 0;
+    for (uint32_t from = first; from < tiles; from += step, side ^= 1) {
+        f32x4 acc[NT][MT];
+        u32x4 now[NT];
+        u32x2 scale[NT][GROUPS];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            now[n] = w[n];
+#pragma unroll
+            for (int q = 0; q < GROUPS; q++) scale[n][q] = sc[n][q];
+#pragma unroll
+            for (int m = 0; m < MT; m++) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        fetch(from + team * NT + step);
+        if (has) {
 #pragma unroll
             for (int q = 0; q < GROUPS; q++) {
                 f32x4 d[NT][MT];
@@ -91,46 +184,38 @@ __global__ __launch_bounds__(512) void k_w4_linear(const T *x, uint64_t x_stride
 #pragma unroll
                     for (int m = 0; m < MT; m++) d[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = q * GS; s < (q + 1) * GS; s++) {
-                    bf16x8 b[MT][XP];
-#pragma unroll
-                    for (int m = 0; m < MT; m++) load_x<T>(x + (uint64_t)min(m0 + 16 * m + col, M - 1) * x_stride, 128 * c + 32 * s + 8 * g, K, vec, b[m]);
+                for (int s = q * GS; s < (q + 1) * GS; s++)
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        const bf16x8 a = codes8(w[n][s]);
+                        const bf16x8 a = codes8(now[n][s]);
 #pragma unroll
                         for (int p = 0; p < XP; p++)
 #pragma unroll
-                            for (int m = 0; m < MT; m++) d[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[m][p], d[n][m], 0, 0, 0);
+                            for (int m = 0; m < MT; m++) d[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[s][m][p], d[n][m], 0, 0, 0);
                     }
-                }
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const f32x4 f = {as_f32(sc[n][q][0] << 16), as_f32(sc[n][q][0] & 0xffff0000u), as_f32(sc[n][q][1] << 16), as_f32(sc[n][q][1] & 0xffff0000u)};
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) acc[n][m][r] = fmaf(f[r], d[n][m][r], acc[n][m][r]);
-                }
+                    for (int m = 0; m < MT; m++) add_scaled(acc[n][m], scale[n][q], d[n][m]);
             }
         }
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int m = 0; m < MT; m++) s_sum[wave][n][m][lane] = acc[n][m];
-    __syncthreads();
-    for (uint32_t i = part; i < NT * MT; i += kw) {
-        const uint32_t n = i / MT, m = i % MT;
-        f32x4 v = s_sum[team * kw][n][m][lane];
-        for (uint32_t o = 1; o < kw; o++) v += s_sum[team * kw + o][n][m][lane];
-        const uint32_t row = m0 + 16 * m + col, out = (tile0 + n) * 16 + 4 * g;
-        if (row >= M) continue;
+            for (int m = 0; m < MT; m++) s_sum[side][wave][n][m][lane] = acc[n][m];
+        __syncthreads();
+        // two neighbouring outputs of a row a thread and turn
+        for (uint32_t i = threadIdx.x; i < teams * NT * MT * 128; i += 512) {
+            const uint32_t half = i & 1, l = (i >> 1) & 63, tm = i >> 7, m = tm % MT, n = tm / MT % NT, t = tm / (MT * NT);
+            f32x2 v = {0.f, 0.f};
+            for (uint32_t o = 0; o < kw; o++) {
+                const f32x4 *p = &s_sum[side][t * kw + o][n][m][l];
+                v += ((const f32x2 *)p)[half];
+            }
+            const uint32_t row = m0 + 16 * m + (l & 15), out = (from + t * NT + n) * 16 + 4 * (l >> 4) + 2 * half;
+            if (row >= M) continue;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            if (out + r >= N) continue;
-            float t = v[r] + (bias ? load1(bias + out + r) : 0.f);
-            if (gelu) t = 0.5f * t * (1.f + erff(t * 0.70710678118654752f));
-            store1(y + (uint64_t)row * N + out + r, t);
+            for (uint32_t r = 0; r < 2; r++) put(v[r], bias, gelu, row, out + r, N, y);
         }
     }
 }
@@ -141,17 +226,29 @@ struct W4Call {
     uint64_t x_stride;
     uint32_t M, N, K, group, vec, gelu, kw;
 };
-template <typename T, int NT, int MT>
-static void launch_w4(hipStream_t st, const W4Call &c)
+template <typename T, int NT, int W>
+static void launch_long(hipStream_t st, const W4Call &c)
 {
-    const uint32_t per = NT * (8 / c.kw);
-    const dim3 grid(((c.N + 15) / 16 + per - 1) / per, (c.M + 16 * MT - 1) / (16 * MT)), block(512);
+    const dim3 grid(((c.N + 15) / 16 + NT - 1) / NT, (c.M + 15) / 16), block(64 * W);
+    auto go = [&](auto k) {
+        hipLaunchKernelGGL(k, grid, block, 0, st, (const T *)c.x, c.x_stride, (const uint32_t *)c.codes, (const uint16_t *)c.scales, (const T *)c.bias, c.M, c.N, c.K, c.vec, c.gelu, (T *)c.y);
+    };
+    if (c.group == 32) go(k_w4_linear_long<T, NT, 1, W>);
+    else if (c.group == 64) go(k_w4_linear_long<T, NT, 2, W>);
+    else go(k_w4_linear_long<T, NT, 4, W>);
+}
+
+template <typename T, int NT, int MT>
+static void launch_many(hipStream_t st, const W4Call &c)
+{
+    const uint32_t per = NT * (8 / c.kw), mb = (c.M + 16 * MT - 1) / (16 * MT), most = std::max(1u, 512 / mb);
+    const dim3 grid(std::min(((c.N + 15) / 16 + per - 1) / per, most), mb), block(512);
     auto go = [&](auto k) {
         hipLaunchKernelGGL(k, grid, block, 0, st, (const T *)c.x, c.x_stride, (const uint32_t *)c.codes, (const uint16_t *)c.scales, (const T *)c.bias, c.M, c.N, c.K, c.kw, c.vec, c.gelu, (T *)c.y);
     };
-    if (c.group == 32) go(k_w4_linear<T, NT, MT, 1>);
-    else if (c.group == 64) go(k_w4_linear<T, NT, MT, 2>);
-    else go(k_w4_linear<T, NT, MT, 4>);
+    if (c.group == 32) go(k_w4_linear_many<T, NT, MT, 1>);
+    else if (c.group == 64) go(k_w4_linear_many<T, NT, MT, 2>);
+    else go(k_w4_linear_many<T, NT, MT, 4>);
 }
 
 template <typename T>
@@ -164,20 +261,25 @@ static int w4_linear(void *stream, const void *x, uint64_t x_stride, const void 
         fmi_set_error("sealnn_w4_linear: K = %u, operands must be given and aligned (codes to 16 bytes, scales to 8)", K);
         return FMI_ERR_ARG;
     }
-    if (N > (1u << 26) || K > (1u << 26) || M > (1u << 20)) { fmi_set_error("sealnn_w4_linear: %u x %u x %u is too large", M, N, K); return FMI_ERR_UNSUPPORTED; }
+    if (N > (1u << 26) || K > (1u << 26) || M > (1u << 19)) { fmi_set_error("sealnn_w4_linear: %u x %u x %u is too large", M, N, K); return FMI_ERR_UNSUPPORTED; }
     const uint32_t vec = ((uintptr_t)x & 15) == 0 && (x_stride * sizeof(T)) % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
-    const uint32_t tiles = (N + 15) / 16, chunks = (K + 127) / 128, kw = chunks >= 8 ? 8 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1;
-    const W4Call c = {x, codes, scales, bias, y, x_stride, M, N, K, group, vec, gelu, kw};
-    // Several tiles a wave share the planes of x, as long as that leaves a workgroup and a half or two for every CU (256 CUs).  us, one tile / several:
-    // 1 x 50265 x 1024 17.8 / 14.5, 1 x 1024 x 1024 4.0 / 5.8, 1 x 50265 x 64 5.0 / 7.6; 64 x 50265 x 1024 fp32 102 / 63, 60 x 4096 x 1024 bf16 7.7 / 6.3, 60 x 1024 x 4096 11.2 / 12.6.
-    // Two tiles of rows: four (64 rows of x at once) are 1.2 to 1.6 times slower, their registers leave one workgroup a CU.
-    const uint64_t teams = 8 / kw;
-    if (M <= 16) {
-        if (tiles >= 512 * 4 * teams) launch_w4<T, 4, 1>(st, c);
-        else launch_w4<T, 1, 1>(st, c);
-    } else if ((uint64_t)tiles * ((M + 31) / 32) >= 256 * 2 * teams) launch_w4<T, 2, 2>(st, c);
-    else launch_w4<T, 1, 2>(st, c);
+    const uint32_t tiles = (N + 15) / 16, chunks = (K + 127) / 128;
+    const W4Call c = {x, codes, scales, bias, y, x_stride, M, N, K, group, vec, gelu, chunks > 4 ? 8u : chunks > 2 ? 4u : chunks};
+    // Measured (us; M x N x K):
+    //   x in registers against read again for each tile of outputs: 1 x 50265 x 1024 11.0 / 14.5, 64 x 50265 x 1024 fp32 33 / 63, 1 x 1024 x 1024 3.7 / 4.0.
+    //   one tile a wave / two, where every CU has one anyway or not: 1 x 1024 x 1024 3.7 / 4.4, 4 x 4096 x 1024 3.9 / 4.2; 1 x 16384 x 1024 6.0 / 5.8,
+    //   32 x 3000 x 1024 7.4 / 5.9, 64 x 50265 x 1024 36 / 33; four: 1 x 50265 x 1024 15.5.
+    //   16 rows of x a wave / 32: fp32, whose planes take three times the registers, 64 x 50265 x 1024 33 / 37; bf16 27 / 24, 60 x 4096 x 1024 6.7 / 5.8, but 60 x 1024 x 1024 3.8 / 5.5.
+    //   more than 1024 columns, one tile / four: 1 x 1024 x 4096 6.2 / 11.8, 4 x 4096 x 2048 5.0 / 7.4; 40 x 24000 x 2000 bf16 32.9 / 23.1, 64 x 12000 x 4096 fp32 95 / 38.
+    //   (32 rows a wave there: 50 to 97.)
+    const uint64_t tiles16 = (uint64_t)tiles * ((M + 15) / 16), tiles32 = (uint64_t)tiles * ((M + 31) / 32);
+    if (chunks <= 8) {
+        if (std::is_same<T, bf16>::value && M > 16 && tiles32 >= 512) launch_many<T, 2, 2>(st, c);
+        else if (tiles16 > 256) launch_many<T, 2, 1>(st, c);
+        else launch_many<T, 1, 1>(st, c);
+    } else if (tiles16 >= 1024) launch_long<T, 4, 8>(st, c);
+    else launch_long<T, 1, 16>(st, c);
     NNCHK();
     return FMI_OK;
 }

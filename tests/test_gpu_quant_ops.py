@@ -57,7 +57,8 @@ def _product_bound(x, w, y, K, dt):
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("M,N,K,group", [(1, 16, 128, 32), (1, 1, 1, 32), (1, 50, 7, 64), (2, 33, 129, 128), (3, 64, 256, 64), (15, 100, 1000, 32), (16, 48, 1024, 128),
                                          (17, 1000, 384, 32), (33, 17, 640, 64), (60, 96, 1030, 32), (64, 31, 128, 128), (65, 40, 260, 64), (130, 16, 512, 32),
-                                         (1, 20000, 96, 64), (5, 300, 4096, 32)])
+                                         (1, 20000, 96, 64), (5, 300, 4096, 32), (2, 50265, 640, 64), (40, 50000, 500, 32), (17, 9000, 130, 128), (70, 8200, 65, 32),
+                                         (3, 17000, 1100, 64), (40, 8200, 1500, 128)])
 def test_product(M, N, K, group, dt):
     g = torch.Generator().manual_seed(M * 7 + N * 3 + K)
     w = quantize_w4(torch.randn(N, K, generator=g), group)

@@ -137,7 +137,7 @@ def test_c_entries_refuse_before_they_launch():
         ap, at, sm = getattr(L, "sealnn_kv8_append" + sfx), getattr(L, "sealnn_kv8_attend" + sfx), getattr(L, "sealnn_sample_tokens" + sfx)
         bad = [lambda: w4(None, p, 128, p, p, None, 1, 16, 128, 48, 0, p), lambda: w4(None, None, 128, p, p, None, 1, 16, 128, 32, 0, p),
                lambda: w4(None, p, 128, p + 4, p, None, 1, 16, 128, 32, 0, p), lambda: w4(None, p, 128, p, p, None, 1, 16, 0, 32, 0, p),
-               lambda: w4(None, p + 1, 128, p, p, None, 1, 16, 128, 32, 0, p), lambda: w4(None, p, 128, p, p, None, 1 << 21, 16, 128, 32, 0, p),
+               lambda: w4(None, p + 1, 128, p, p, None, 1, 16, 128, 32, 0, p), lambda: w4(None, p, 128, p, p, None, (1 << 19) + 1, 16, 128, 32, 0, p),
                lambda: ap(None, p, p, st, 1, p, None, p, p, p, p, 1, 1, 64, 16, 32), lambda: ap(None, p, p, st, 1, p, None, p, p, p, p, 1, 1, 65, 16, 64),
                lambda: ap(None, p, p, st, 1, p, None, p, p, p, p, 1, 1, 64, 24, 64), lambda: ap(None, p, p, st, 1, None, None, p, p, p, p, 1, 1, 64, 16, 64),
                lambda: ap(None, p, p, st, 1, p, None, p + 8, p, p, p, 1, 1, 64, 16, 64), lambda: ap(None, p, None, st, 1, p, None, p, p, p, p, 1, 1, 64, 16, 64),
