@@ -59,6 +59,7 @@ struct Shared {
     uint64_t list[LIST];                                 // (key << 32 | ~index) of the tokens that matter: falling order = falling logit, equal ones by rising index
     uint64_t order[LIST];                                // those of them that a border falls between
     uint64_t part[MAX_VOCAB / 256];                      // weights of 256 consecutive tokens each
+    float top[MAX_VOCAB / STRIPE / 4 * WAVES];           // the largest that may be drawn of a wave's tokens in four stripes
     uint64_t wave[WAVES];
     float wavef[2 * WAVES];
     double root[32];                                     // 2^(i / 32)
@@ -411,9 +412,13 @@ __global__ __launch_bounds__(256) void k_sample_lists(SampleArgs a)
         if (entry[i]) { if (at < LIST) out.list[at] = entry[i]; at++; }
 }
 
-// One workgroup per row.  The row is read for the maxima, then once more (from the caches): for the sum of exponentials, the weights where a nucleus needs
-// their total, and a list of the largest tokens -- those that reach the k-th largest (top-k) or the 768th largest (a nucleus) of the threads' own
-// maxima.  Where the list holds what the filters leave, everything else happens on it; otherwise the filters read the row again.
+// One workgroup per row.  The row is read for the maxima and the sum of exponentials, then once more: for a list of the largest tokens -- those that reach the k-th
+// largest (top-k) or the 768th largest (a nucleus of all) of the threads' own maxima, or min_p of the largest weight -- and the weights where a nucleus needs
+// their total.  Of the second reading a wave leaves out what its maxima show to be below.  Where the list holds what the filters leave, everything else
+// happens on it; otherwise they read the row again.  SPLIT: the two kernels before this one have read the row already.
+// Bound by instructions and waiting, not by memory: 512 rows of 131072 bf16 under min_p 55 us (2.4 TB/s; 83 with the weights taken four a lane in the second
+// reading instead of from the list), 300 rows of 50265 fp32 under a bitmap, top-k and top-p 39 us (the 44 rows beyond one for every CU cost 14 of them), a nucleus
+// of all 69 (its 50265 weights in 64 bits).  Eight waves a SIMD: a workgroup of 16 waves more to hide a row's latency behind, for 4 to 14 spilled registers.
 template <typename T, bool BITS, bool SPLIT>
 __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(SampleArgs a)
 {
@@ -423,22 +428,46 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
     const Row<T, BITS> x(a, row);
     typedef typename Row<T, BITS>::Raw Raw;
     const uint32_t stripes = (V + STRIPE - 1) / STRIPE;
-    auto row_pass = [&](auto f) {                                // f(index of the first, four logits, which may be drawn)
+    // Stripes of the row (a bit each), four of them in flight: f(the stripes, how many, indices of the first logits, four logits each, which may be drawn)
+    static_assert(MAX_VOCAB <= 64 * STRIPE, "a bit for each stripe");
+    auto stripe_pass = [&](uint64_t mask, auto f) {
         enum { FLY = 4 };
-        for (uint32_t i0 = 0; i0 < stripes; i0 += FLY) {
+        while (mask) {
+            uint32_t at[FLY], n = 0;
             Raw w[FLY];
             uint32_t b[FLY];
 #pragma unroll
-            for (uint32_t j = 0; j < FLY; j++) { const uint32_t i = min(i0 + j, stripes - 1); w[j] = x.load(i, tid); b[j] = x.load_bits(i, tid); }
+            for (uint32_t j = 0; j < FLY; j++) {
+                at[j] = mask ? (uint32_t)__ffsll((unsigned long long)mask) - 1 : at[j ? j - 1 : 0];
+                n += mask != 0;
+                mask &= mask - 1;
+                w[j] = x.load(at[j], tid);
+                b[j] = x.load_bits(at[j], tid);
+            }
+            float v[FLY][4];
+            uint32_t ok[FLY];
 #pragma unroll
-            for (uint32_t j = 0; j < FLY; j++)
-                if (i0 + j < stripes) { float v[4]; const uint32_t ok = x.unpack(i0 + j, tid, w[j], b[j], v); f((i0 + j) * STRIPE + 4 * tid, v, ok); }
+            for (uint32_t j = 0; j < FLY; j++) ok[j] = x.unpack(at[j], tid, w[j], b[j], v[j]);
+            f(at, n, v, ok);
         }
     };
+    const uint64_t every = stripes < 64 ? ((uint64_t)1 << stripes) - 1 : ~(uint64_t)0;
+    // the wave's stripes, four by four, with a token that may be drawn of at least `from`
+    const Settings set(a, row);
+    const bool skips = !SPLIT && (set.has_k || (!set.has_p && set.min_p > 0.f));     // (a nucleus of all weighs every token, and without a filter every token stays)
+    auto stripes_from = [&](float from) -> uint64_t { return !skips ? every : __ballot(lane < stripes && s.top[lane / 4 * WAVES + wave] >= from); };
+    auto row_pass = [&](uint64_t mask, auto f) {                 // f(index of the first, four logits, which may be drawn)
+        stripe_pass(mask, [&](const uint32_t *at, uint32_t n, float (*v)[4], const uint32_t *ok) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) if (j < n) f(at[j] * STRIPE + 4 * tid, v[j], ok[j]);
+        });
+    };
+    const float L2E = 1.4426950408889634f, LOWEST = -3.402823466e38f;
     if (tid < 32) s.root[tid] = exp2((double)tid / 32.0);
     // the largest logit, and the largest that may be drawn (fmaxf leaves NaN out)
-    const float L2E = 1.4426950408889634f;
     float mx = NINF, mz = NINF, own = NINF;                      // own: the thread's largest that may be drawn
+    float z = 0.f;                                               // the sum of exponentials against `base` (fp32: it enters the log-probabilities only)
+    double base;
     Record rec;
     uint64_t part = 0;
     uint32_t on_list = 0;
@@ -451,27 +480,91 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
         s.list[tid] = in.list[tid];                              // (all of it: its length is on its way, too)
         s.list[tid + THREADS] = in.list[tid + THREADS];
         row_maxima(rec, s.wavef, lane, wave, mx, mz);
+        z = rec.z * __builtin_amdgcn_exp2f((rec.max - mx) * L2E);
+        base = (double)mx;
     } else {
-        row_pass([&](uint32_t, const float *v, uint32_t ok) {
+        // On the values as they are, 16 a thread and turn; NaN comes through a maximum, and with anything beyond +-1e30 it is for the careful loops below.  The sum of
+        // exponentials is taken against `ref` in the exponent of 2, so that x log2(e) - ref is one instruction and rounds once.
+        float ref = -1.5e30f;
+        stripe_pass(every, [&](const uint32_t *at, uint32_t n, float (*v)[4], const uint32_t *ok) {
+            float top = NINF;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                mx = fmaxf(mx, v[e]);
-                if (BITS) mz = fmaxf(mz, (ok >> e) & 1 ? v[e] : NINF);
-            }
+            for (uint32_t j = 0; j < 4; j++)
+                if (j < n) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        mx = __builtin_elementwise_maximum(mx, v[j][e]);
+                        if (BITS) top = __builtin_elementwise_maximum(top, as_f32((ok[j] >> e) & 1 ? as_u32(v[j][e]) : 0xff800000u));
+                    }
+                }
+            const float to = fmaxf(mx, -1e30f) * L2E;
+            z *= __builtin_amdgcn_exp2f(ref - to);
+            ref = to;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++)
+                if (j < n) {
+                    if (!BITS) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) top = __builtin_elementwise_maximum(top, v[j][e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z += __builtin_amdgcn_exp2f(fmaf(v[j][e], L2E, -to));
+                }
+            own = __builtin_elementwise_maximum(own, top);
+            if (!skips) return;
+            top = wave_max(top);
+            if (lane == 0) s.top[at[0] / 4 * WAVES + wave] = top;
         });
-        own = clean(BITS ? mz : mx);
+        const bool wild = __any(!(mx <= 1e30f) || (mx < -1e30f && mx > NINF));
         mx = wave_max(mx);
-        mz = BITS ? wave_max(mz) : mx;
-        if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; }
+        mz = wave_max(own);
+        if (lane == 0) { s.wavef[wave] = wild ? __builtin_nanf("") : mx; s.wavef[WAVES + wave] = mz; }
         __syncthreads();
-        mx = clean(wave_max(s.wavef[lane % WAVES]));
-        mz = clean(wave_max(s.wavef[WAVES + lane % WAVES]));
+        mx = s.wavef[lane % WAVES];
+        mz = wave_max(s.wavef[WAVES + lane % WAVES]);
+        if (!__any(mx != mx)) {
+            mx = wave_max(mx);
+            const float to = mx * L2E;
+            z *= __builtin_amdgcn_exp2f(ref - to);
+            base = (double)to / (double)L2E;
+        } else {
+            z = 0.f;
+            mx = own = NINF;
+            stripe_pass(every, [&](const uint32_t *at, uint32_t n, float (*v)[4], const uint32_t *ok) {
+                float top = NINF;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+                    if (j < n) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float c = clean(v[j][e]);
+                            mx = fmaxf(mx, c);
+                            if (!BITS || ((ok[j] >> e) & 1)) top = fmaxf(top, c);
+                        }
+                    }
+                own = fmaxf(own, top);
+                if (!skips) return;
+                top = wave_max(top);
+                if (lane == 0) s.top[at[0] / 4 * WAVES + wave] = top;
+            });
+            mx = wave_max(mx);
+            mz = wave_max(own);
+            __syncthreads();
+            if (lane == 0) { s.wavef[wave] = mx; s.wavef[WAVES + wave] = mz; }
+            __syncthreads();
+            mx = wave_max(s.wavef[lane % WAVES]);
+            mz = wave_max(s.wavef[WAVES + lane % WAVES]);
+            base = (double)mx;
+            row_pass(every, [&](uint32_t, const float *v, uint32_t) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) z += __builtin_amdgcn_exp2f((clean(v[e]) - mx) * L2E);
+            });
+        }
     }
     if (mz == NINF) {                                            // nothing may be drawn
         for (uint32_t d = tid; d < a.draws; d += THREADS) { a.tokens[(uint64_t)row * a.draws + d] = -1; a.logprobs[(uint64_t)row * a.draws + d] = NINF; }
         return;
     }
-    const Settings set(a, row);
     const Scale sc(set, mz);
     auto weigh = [&](float v) { return weight(v, sc.m, sc.inv, s.root); };
     auto one = [](float) { return 1.0; };
@@ -479,29 +572,18 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
     auto value_of = [](uint64_t e) { const uint32_t k = (uint32_t)(e >> 32); return as_f32((k >> 31) ? k ^ 0x80000000u : ~k); };
     uint32_t thr = 0, lim = 0xffffffffu;                         // kept: key > thr, or key == thr and index <= lim
     auto kept = [&](float v, uint32_t idx) { const uint32_t k = key_of(v); return k > thr || (k == thr && idx <= lim); };
-    // The sum of exponentials over the whole row (fp32: it enters the log-probabilities only), added up by the first pass behind the maxima; v cleaned
-    float z = 0.f;
-    bool have_z = SPLIT;
-    if (SPLIT && rec.max > NINF) z = rec.z * __builtin_amdgcn_exp2f((rec.max - mx) * L2E);
-    auto add_z = [&](const float *v) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) z += __builtin_amdgcn_exp2f((v[e] - mx) * L2E);
-    };
-    // every token that may be drawn and is at least `from`: f(cleaned logit, index); also(four cleaned logits, which may be drawn)
-    auto row_from = [&](float from, auto f, auto also) {
-        row_pass([&](uint32_t at, float *v, uint32_t ok) {
+    // every token that may be drawn and is at least `from`: f(logit, index)
+    auto row_from = [&](float from, auto f) {
+        row_pass(stripes_from(from), [&](uint32_t at, float *v, uint32_t ok) {
             bool any = false;
 #pragma unroll
-            for (int e = 0; e < 4; e++) { v[e] = clean(v[e]); any |= v[e] >= from; }
-            also(v, ok);
+            for (int e = 0; e < 4; e++) any |= v[e] >= from;
             if (any) {
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) if (v[e] >= from && (!BITS || ((ok >> e) & 1))) f(v[e], at + e);
+                for (uint32_t e = 0; e < 4; e++) if (v[e] >= from && (!BITS || ((ok >> e) & 1))) f(clean(v[e]), at + e);
             }
         });
     };
-    const float LOWEST = -3.402823466e38f;                       // (a logit of -inf is never drawn)
-    auto nothing = [](const float *, uint32_t) {};
     auto clear_buckets = [&]() {
         __syncthreads();
         s.mass[tid] = s.mass[tid + THREADS] = 0;
@@ -510,6 +592,7 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
     };
     uint32_t listed = 0;                                         // > 0: everything that is kept is among the list's first entries (in no order)
     auto list_pass = [&](auto f) { for (uint32_t i = tid; i < listed; i += THREADS) f(value_of(s.list[i]), ~(uint32_t)s.list[i]); };
+    auto put_list = [&](float v, uint32_t idx) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LIST) s.list[at] = ((uint64_t)key_of(v) << 32) | (uint32_t)~idx; };
     auto put_order = [&](float v, uint32_t idx) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LIST) s.order[at] = ((uint64_t)key_of(v) << 32) | (uint32_t)~idx; };
 
     // The border inside s.order[0 .. n), all of it kept so far, behind a sum of `front`: thr and lim become the first token (in order) whose running sum
@@ -625,12 +708,7 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
         __syncthreads();
         return true;
     };
-    auto row_all = [&](auto f) {
-        const bool with_z = !have_z;
-        have_z = true;
-        row_from(LOWEST, f, [&](const float *v, uint32_t) { if (with_z) add_z(v); });
-    };
-
+    auto row_all = [&](auto f) { row_from(LOWEST, f); };        // (a logit of -inf is never drawn)
     const bool has_k = set.has_k, has_p = set.has_p;
     const uint64_t k = (uint64_t)set.top_k;
     const double p = (double)fmaxf(set.top_p, 0.f);
@@ -655,19 +733,23 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
             __syncthreads();
             from = value_of((uint64_t)s.kmin << 32);
         }
-        have_z = true;
         __syncthreads();
-        row_from(from, [&](float v, uint32_t idx) { const uint32_t at = atomicAdd(&s.n, 1u); if (at < LIST) s.list[at] = ((uint64_t)key_of(v) << 32) | (uint32_t)~idx; },
-                 [&](const float *v, uint32_t ok) {
-                     add_z(v);
-                     if (!has_k) {
-#pragma unroll
-                         for (int e = 0; e < 4; e++) if (!BITS || ((ok >> e) & 1)) own_mass += weigh(v[e]);
-                     }
-                 });
+        if (has_k) row_from(from, put_list);
+        else
+            row_from(LOWEST, [&](float v, uint32_t idx) {
+                own_mass += weigh(v);
+                if (v >= from) put_list(v, idx);
+            });
         __syncthreads();
         listed = s.n <= LIST ? s.n : 0;
         if (!has_k) { block_scan((uint64_t)own_mass, s, lane, wave, total); }
+        __syncthreads();
+    } else if (skips && !has_k) {                                // min_p alone: the tokens that it leaves, if they fit
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        row_from(sc.low, put_list);
+        __syncthreads();
+        listed = s.n <= LIST ? s.n : 0;
         __syncthreads();
     }
     if (has_k) {
@@ -727,15 +809,14 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
     if (SPLIT && !has_k && !has_p) {}
     else if (listed) list_pass([&](float v, uint32_t idx) { const uint64_t w = final_weight(v, idx); if (w) atomicAdd((unsigned long long *)&s.part[idx >> 8], (unsigned long long)w); });
     else
-        row_pass([&](uint32_t at, float *v, uint32_t ok) {
+        row_pass(stripes_from(low), [&](uint32_t at, float *v, uint32_t ok) {
             uint64_t w = 0;
             bool any = false;
 #pragma unroll
-            for (int e = 0; e < 4; e++) { v[e] = clean(v[e]); any |= v[e] >= low; }
-            if (!have_z) add_z(v);
+            for (int e = 0; e < 4; e++) any |= v[e] >= low;
             if (any) {
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) if (!BITS || ((ok >> e) & 1)) w += final_weight(v[e], at + e);
+                for (uint32_t e = 0; e < 4; e++) if (!BITS || ((ok >> e) & 1)) w += final_weight(clean(v[e]), at + e);
             }
             if (__any(w != 0)) {
                 const uint64_t sum = wave_scan(w);
@@ -753,7 +834,7 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
     if (wave >= a.draws) return;
     double lse = 0.0;
     for (int w = 0; w < WAVES; w++) lse += (double)s.wavef[w];
-    lse = (double)mx + log(lse);
+    lse = base + log(lse);
     for (uint32_t d = wave; d < a.draws; d += WAVES) {
         // floor(u * left), and the first 256 tokens whose running sum passes it
         const float u = a.u[(uint64_t)row * a.draws + d];
