@@ -924,12 +924,12 @@ def main():
         dist.init_process_group("nccl", device_id=dev, rank=rank, world_size=world)
 
     import __graft_entry__ as ge
-    from seal_amd import FMIndex
+    from seal_amd import FMIndex, _build
     from seal_amd._lib import check, lib
     from seal_amd.retrieval import SEALSearcher
     from seal_amd import retrieval, keys as rk
     from seal_amd.distributed import gather_topk, pack_topk
-    if rank == 0:
+    if rank == 0 and _build.stale():           # (what is built is loaded)
         ge.build()
     if use_dist:
         dist.barrier()
