@@ -12,8 +12,9 @@ from ._lib import launch, lib, uint64s
 
 TILE = 64                                  # tokens of a tile of the layout
 # Workgroups (of four waves) that a call splits long slots into when it has few: one a CU is enough for many items (32 slots x 8 heads of up to 8192 tokens: 79 us, in two
-# parts 84), two a CU are better where every item is split anyway (1 slot x 16 heads of 32001 tokens: 16 parts 19.0 us, 32 18.0, 64 19.3)
-ITEMS_ENOUGH, PARTS_WANTED = 256, 512
+# parts 84), two a CU are better where every item is split anyway (1 slot x 16 heads of 32001 tokens: 16 parts 19.0 us, 32 18.0, 64 19.3).  Short caches are not split: the
+# second launch and the workspace cost a caller 4 us (1 slot x 16 heads of 512 tokens: 8.3 us a call, split 12.2; in a graph 6.5 / 7.5; of 2048 tokens 16.0 / 12.1, 15.7 / 8.1)
+ITEMS_ENOUGH, PARTS_WANTED, SPLIT_TOKENS = 256, 512, 1024
 
 
 class KV8Cache:
@@ -101,7 +102,7 @@ class KV8Cache:
         lengths_ptr, index = self._lengths(lengths, "lengths"), self._on_gpu()
         out = q.new_empty(shape)
         items = self.slots * H * ((beams * share + 15) // 16)
-        splits = 1 if items >= ITEMS_ENOUGH or not items else max(1, min(self.tokens // TILE // 4, PARTS_WANTED // items))
+        splits = 1 if self.tokens < SPLIT_TOKENS or items >= ITEMS_ENOUGH or not items else max(1, min(self.tokens // TILE // 4, PARTS_WANTED // items))
         work, work_floats = None, 0
         if splits > 1:
             work_floats = shape[0] * shape[1] * splits * (D + 4)
