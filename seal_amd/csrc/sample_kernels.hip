@@ -97,8 +97,9 @@ static __device__ __forceinline__ uint64_t wave_total(uint64_t scanned)
 {
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(scanned >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)scanned, 63);
 }
+// (NaN comes through: an instruction less a step than a maximum that drops it)
 template <int CTRL, int ROWS> static __device__ __forceinline__ float dpp_max(float v)
-{ return fmaxf(v, as_f32(dpp<CTRL, ROWS>(0xff800000u, as_u32(v)))); }
+{ return __builtin_elementwise_maximum(v, as_f32(dpp<CTRL, ROWS>(0xff800000u, as_u32(v)))); }
 static __device__ __forceinline__ float wave_max(float v)
 {
     v = dpp_max<0x111, 0xf>(v); v = dpp_max<0x112, 0xf>(v); v = dpp_max<0x114, 0xf>(v); v = dpp_max<0x118, 0xf>(v);
