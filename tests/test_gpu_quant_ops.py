@@ -400,9 +400,11 @@ def test_sample_spread_over_the_card_draws_the_same_tokens(V, dt, monkeypatch):
     few = torch.rand(len(rows), V, generator=g) < 2e-3
     few[5, 1:] = False
     few[5, 0] = True
+    own = dict(temperature=torch.tensor([1.0, 0.5, 0.0, 1.3, 0.8, 2.0, 1.0], device=DEV), top_k=torch.tensor([0, 513, 5, 0, 40, -1, 512], dtype=torch.int32, device=DEV),
+               top_p=torch.tensor([1.0, 0.9, 0.2, 0.6, 0.95, 1.0, 0.0], device=DEV), min_p=torch.tensor([0.0, 0.0, 0.5, 0.1, 0.01, 0.02, 0.0], device=DEV))
     for bits in (None, _pack(few).to(DEV)):
         for kw in (dict(), dict(min_p=0.1), dict(top_p=0.9), dict(top_p=0.999, temperature=1.4), dict(top_k=1), dict(top_k=60), dict(top_k=512, top_p=0.7), dict(top_k=513),
-                   dict(top_k=V - 1, top_p=0.5, min_p=0.001), dict(temperature=0.0)):
+                   dict(top_k=V - 1, top_p=0.5, min_p=0.001), dict(temperature=0.0), own):
             monkeypatch.undo()
             spread = sample_tokens(x, u, allowed_bits=bits, **kw)
             monkeypatch.setattr("seal_amd.sampling.SPLIT_ROWS", 0)
@@ -431,6 +433,29 @@ def test_sample_values_that_are_not_finite():
     none = torch.ones(8, V, dtype=torch.bool)
     none[2:4] = False
     assert (_check_samples(x, u, allowed=none, top_p=0.5)[2:4] == -1).all()
+
+
+@pytest.mark.parametrize("V", [20000, 40000])
+def test_sample_values_that_are_not_finite_in_long_rows(V):
+    """the same in rows of several turns, and numbers beyond 1e30 of either sign"""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(8, V, generator=g) * 3
+    x[0, ::777] = float("nan")
+    x[1, [17, V - 2]] = float("inf")
+    x[2, :] = -float("inf")
+    x[2, [3, 9000, V - 1]] = torch.tensor([0.5, 1.0, 0.25])
+    x[3] = -2e30 + x[3] * 1e28
+    x[4, 12345] = 2e30
+    x[5, ::2] = -float("inf")
+    x[6, :] = float("nan")
+    x[6, 8191] = 2.0
+    x[7, :] = float("nan")
+    u = torch.rand(8, 3, generator=g)
+    allowed = torch.rand(8, V, generator=g) < 0.3
+    allowed[2, 9000] = allowed[6, 8191] = True
+    for kw in (dict(), dict(top_k=5, top_p=0.9), dict(top_p=0.5), dict(min_p=0.05), dict(temperature=0.0)):
+        assert (_check_samples(x, u, **kw)[7] == -1).all()
+        assert (_check_samples(x, u, allowed=allowed, **kw)[7] == -1).all()
 
 
 def test_sample_settings_row_by_row_and_strides():
