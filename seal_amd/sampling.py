@@ -11,7 +11,9 @@ from ._lib import launch, lib
 
 MAX_VOCAB = 1 << 18
 # Few rows of a large vocabulary are spread over the card by three kernels instead of one workgroup each (include/sealnn.h).  us, one kernel / three, fp32, top-p 0.9: 1 x 16384
-# 22.7 / 23.5, 1 x 50265 36.7 / 24.4, 32 x 50265 38 / 28, 128 x 50265 40.5 / 41.8, 1 x 131072 60.7 / 25.0; top-k 50: 1 x 50265 19.2 / 20.5, 64 x 50265 21.4 / 26.5, 1 x 131072 26.1 / 20.4
+# 24.1 / 23.6, 1 x 50265 39.7 / 24.7, 32 x 50265 41 / 28, 128 x 50265 42.6 / 42.1, 1 x 131072 66 / 25; top-k 50: 1 x 50265 20.6 / 20.8, 32 x 131072 27.7 / 27.6, 128 x 50265 23 / 32
+# (where every token has to be weighed -- no top-k, no min-p -- it pays up to twice the rows: 64 x 50265 top-p 0.9 41.5 / 34.1, without a filter 34.8 / 24.1,
+# under a bitmap 28.6 / 28.6, but 128 x 50265 under a bitmap 29.4 / 35.3)
 SPLIT_VOCAB, SPLIT_ROWS = 32768, 32
 Setting = Union[float, int, torch.Tensor]
 
@@ -89,7 +91,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
         raise RuntimeError("sample_tokens: the logits must live on the GPU (seal_amd has no CPU path)")
     tokens, logprobs = u.new_empty(u_shape, dtype=torch.int64), u.new_empty(u_shape)
     work, work_bytes = None, 0
-    if vocab >= SPLIT_VOCAB and rows <= SPLIT_ROWS:
+    if vocab >= SPLIT_VOCAB and rows <= (SPLIT_ROWS if k or m or k_v is not None or m_v is not None or (t_v is None and not t) else 2 * SPLIT_ROWS):
         work_bytes = rows * (-(-vocab // 1024) * 96 + 16448)
         work = torch.empty(work_bytes, dtype=torch.uint8, device=dev)
     launch(lib().sealnn_sample_tokens if dt == torch.float32 else lib().sealnn_sample_tokens_bf16, logits.get_device(), logits.data_ptr(), row_stride, rows, vocab,
