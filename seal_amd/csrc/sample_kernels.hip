@@ -241,20 +241,26 @@ struct Settings {
     __device__ __forceinline__ bool lists() const { return has_k ? (uint32_t)top_k <= THREADS / 2 : has_p; }
 };
 
+// what is the same in every lane, out of the vector registers (a row's constants would fill a quarter of them)
+static __device__ __forceinline__ float uniform(float v) { return as_f32((uint32_t)__builtin_amdgcn_readfirstlane((int)as_u32(v))); }
+static __device__ __forceinline__ double uniform(double v)
+{ return __hiloint2double(__builtin_amdgcn_readfirstlane(__double2hiint(v)), __builtin_amdgcn_readfirstlane(__double2loint(v))); }
+
 // How a row's logits become weights and buckets; mz: the largest that may be drawn
 struct Scale {
     double m, inv, floor_w;
     float mz, c, low;
-    __device__ __forceinline__ Scale(const Settings &t, float mz_) : mz(mz_)
+    __device__ __forceinline__ Scale(const Settings &t, float mz_)
     {
-        m = (double)mz;
-        inv = 1.4426950408889634074 / (double)t.temperature;
+        mz = uniform(mz_);
+        m = uniform((double)mz);
+        inv = uniform(1.4426950408889634074 / (double)t.temperature);
         // buckets of 1 / 64 of a temperature below the largest logit: they order as the logits do (a rounded difference and product are monotone)
-        c = fminf(64.f / t.temperature, 1e30f);
+        c = uniform(fminf(64.f / t.temperature, 1e30f));
         // a logit below `low` has no weight: less than min_p of the largest, or 2^-45
-        floor_w = t.min_p > 0.f ? (double)t.min_p * 17592186044416.0 : 0.0;
+        floor_w = uniform(t.min_p > 0.f ? (double)t.min_p * 17592186044416.0 : 0.0);
         const float reach = mz - t.temperature * fminf(31.5f, t.min_p > 0.f ? 1e-3f - 0.69314718f * __builtin_amdgcn_logf(t.min_p) : 31.5f) * 1.00001f;
-        low = fmaxf(reach, -3.402823466e38f);
+        low = uniform(fmaxf(reach, -3.402823466e38f));
     }
     __device__ __forceinline__ uint32_t bucket(float v) const { const float b = (mz - v) * c; return b < (float)(BUCKETS - 1) ? (uint32_t)b : (uint32_t)(BUCKETS - 1); }
 };
@@ -418,8 +424,8 @@ __global__ __launch_bounds__(256) void k_sample_lists(SampleArgs a)
 // their total.  Of the second reading a wave leaves out what its maxima show to be below.  Where the list holds what the filters leave, everything else
 // happens on it; otherwise they read the row again.  SPLIT: the two kernels before this one have read the row already.
 // Bound by instructions and waiting, not by memory: 512 rows of 131072 bf16 under min_p 55 us (2.4 TB/s; 83 with the weights taken four a lane in the second
-// reading instead of from the list), 300 rows of 50265 fp32 under a bitmap, top-k and top-p 39 us (the 44 rows beyond one for every CU cost 14 of them), a nucleus
-// of all 69 (its 50265 weights in 64 bits).  Eight waves a SIMD: a workgroup of 16 waves more to hide a row's latency behind, for 4 to 14 spilled registers.
+// reading instead of from the list), 300 rows of 50265 fp32 under a bitmap, top-k and top-p 34 us (the 44 rows beyond one for every CU cost 10 of them), a nucleus
+// of all 69 (its 50265 weights in 64 bits).  Eight waves a SIMD: a workgroup of 16 waves more to hide a row's latency behind, for 4 to 18 spilled registers.
 template <typename T, bool BITS, bool SPLIT>
 __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(SampleArgs a)
 {
@@ -527,7 +533,7 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
             mx = wave_max(mx);
             const float to = mx * L2E;
             z *= __builtin_amdgcn_exp2f(ref - to);
-            base = (double)to / (double)L2E;
+            base = uniform((double)to / (double)L2E);
         } else {
             z = 0.f;
             mx = own = NINF;
@@ -753,16 +759,67 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
         listed = s.n <= LIST ? s.n : 0;
         __syncthreads();
     }
+    auto row_lse = [&]() {                                       // of the waves' sums in s.wavef
+        double sum = 0.0;
+        for (int w = 0; w < WAVES; w++) sum += (double)s.wavef[w];
+        return base + log(sum);
+    };
+    auto put_z = [&]() {
+        float sum = z;
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == 0) s.wavef[wave] = sum;
+    };
+    // floor(u * all), u as 63 bits
+    auto target_of = [](float u, uint64_t all) -> uint64_t {
+        const double uc = u > 0.f ? fmin((double)u, 1.0 - 1.0 / 16777216) : 0.0;
+        const uint64_t u63 = (uint64_t)(uc * 9223372036854775808.0);
+        return (__umul64hi(u63, all) << 1) | ((u63 * all) >> 63);
+    };
+    if (listed && listed <= 64) {
+        // One wave does what is left, a token a lane: in falling order for the filters, then in the order of the vocabulary for the draws (300 rows of 50265 under
+        // a bitmap with top-k 50 and top-p: 34 us, 39 with the general steps below)
+        put_z();
+        if (tid == 0) s.found = 0;
+        __syncthreads();
+        if (wave == 0) {
+            const uint64_t e = sort_wave(lane < listed ? s.list[lane] : 0, lane);
+            const float v = value_of(e);
+            bool in = lane < listed && (!has_k || lane < k);
+            const double w = in ? weigh(v) : 0.0;
+            bool enough = true;
+            if (has_p) {
+                const uint64_t run = wave_scan((uint64_t)w), all = has_k ? wave_total(run) : total;
+                const uint64_t hit = __ballot(in && run > 0 && (double)run >= p * (double)all);
+                enough = hit != 0;
+                in = in && lane < (uint32_t)__ffsll((unsigned long long)hit);
+            }
+            in = in && v >= sc.low && w >= sc.floor_w;
+            if (enough) {
+                if (lane == 0) s.found = 1;
+                const uint64_t by_index = sort_wave((e << 32) | lane, lane);         // (the low half of an entry is ~index)
+                const int from = (int)(by_index & 63);
+                const uint32_t idx = ~(uint32_t)(by_index >> 32);
+                const float x_at = __shfl(v, from);
+                const uint64_t incl = wave_scan(__shfl(in ? (uint64_t)w : 0, from)), left = wave_total(incl);
+                const double lse = row_lse();
+                for (uint32_t d = 0; d < a.draws; d++) {
+                    const uint64_t target = target_of(a.u[(uint64_t)row * a.draws + d], left), hit = __ballot(incl > target);
+                    if (lane + 1 == (uint32_t)__ffsll((unsigned long long)hit)) {
+                        a.tokens[(uint64_t)row * a.draws + d] = idx;
+                        a.logprobs[(uint64_t)row * a.draws + d] = (float)((double)x_at - lse);
+                    }
+                }
+            }
+        }
+        if (has_k || !has_p) return;                             // (a nucleus of all may be larger than the list)
+        __syncthreads();
+        if (s.found) return;
+        __syncthreads();
+    }
     if (has_k) {
         auto reached = [&](uint64_t f) { return f >= k; };
         if (!listed) shorten(row_all, one, reached);
-        else if (listed <= 64) {
-            if (listed >= k) {                                   // (fewer: the list is everything that may be drawn)
-                if (tid < listed) s.order[tid] = s.list[tid];
-                __syncthreads();
-                border(listed, 0, one, reached);
-            }
-        } else shorten(list_pass, one, reached);
+        else shorten(list_pass, one, reached);
     }
     if (has_p) {
         // (a prefix of mass f is long enough; an empty one never is)
@@ -777,19 +834,6 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
         }
         bool done = false;
         if (listed > 64) done = shorten(list_pass, weigh, reached);
-        else if (listed) {
-            // (few: one wave sorts them all; those that top-k left out become NaN, weigh nothing and sort behind)
-            own_mass = 0.0;
-            list_pass([&](float v, uint32_t idx) { if (kept(v, idx)) own_mass += weigh(v); });
-            uint64_t there;
-            block_scan((uint64_t)own_mass, s, lane, wave, there);
-            done = reached(there);
-            if (done) {
-                if (tid < listed) s.order[tid] = kept(value_of(s.list[tid]), ~(uint32_t)s.list[tid]) ? s.list[tid] : 0;
-                __syncthreads();
-                border(listed, 0, weigh, reached);
-            }
-        }
         if (!done) {                                             // the nucleus is larger than the list
             listed = 0;
             shorten(row_all, weigh, reached);
@@ -828,20 +872,13 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
     uint64_t left;
     const uint64_t incl = block_scan(tid < parts ? s.part[tid] : 0, s, lane, wave, left);
     s.part[tid] = incl;
-    // ... and the sum of exponentials
-    for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o);
-    if (lane == 0) s.wavef[wave] = z;
+    put_z();
     __syncthreads();
     if (wave >= a.draws) return;
-    double lse = 0.0;
-    for (int w = 0; w < WAVES; w++) lse += (double)s.wavef[w];
-    lse = base + log(lse);
+    const double lse = row_lse();
     for (uint32_t d = wave; d < a.draws; d += WAVES) {
         // floor(u * left), and the first 256 tokens whose running sum passes it
-        const float u = a.u[(uint64_t)row * a.draws + d];
-        const double uc = u > 0.f ? fmin((double)u, 1.0 - 1.0 / 16777216) : 0.0;
-        const uint64_t u63 = (uint64_t)(uc * 9223372036854775808.0);
-        const uint64_t target = (__umul64hi(u63, left) << 1) | ((u63 * left) >> 63);
+        const uint64_t target = target_of(a.u[(uint64_t)row * a.draws + d], left);
         uint32_t lo = 0, hi = parts - 1;
         while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (s.part[mid] > target) hi = mid; else lo = mid + 1; }
         const uint64_t rest = target - (lo ? s.part[lo - 1] : 0);

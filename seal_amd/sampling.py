@@ -11,7 +11,7 @@ from ._lib import launch, lib
 
 MAX_VOCAB = 1 << 18
 # Few rows of a large vocabulary are spread over the card by three kernels instead of one workgroup each (include/sealnn.h).  us, one kernel / three, fp32, top-p 0.9: 1 x 16384
-# 24.1 / 23.6, 1 x 50265 39.7 / 24.7, 32 x 50265 41 / 28, 128 x 50265 42.6 / 42.1, 1 x 131072 66 / 25; top-k 50: 1 x 50265 20.6 / 20.8, 32 x 131072 27.7 / 27.6, 128 x 50265 23 / 32
+# 24.1 / 23.6, 1 x 50265 39.7 / 24.7, 32 x 50265 41 / 28, 128 x 50265 42.6 / 42.1, 1 x 131072 66 / 25; top-k 50: 1 x 50265 16.3 / 15.8, 32 x 50265 17.2 / 17.7, 32 x 131072 23.2 / 22.3
 # (where every token has to be weighed -- no top-k, no min-p -- it pays up to twice the rows: 64 x 50265 top-p 0.9 41.5 / 34.1, without a filter 34.8 / 24.1,
 # under a bitmap 28.6 / 28.6, but 128 x 50265 under a bitmap 29.4 / 35.3)
 SPLIT_VOCAB, SPLIT_ROWS = 32768, 32
