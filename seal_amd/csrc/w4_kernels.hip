@@ -44,6 +44,35 @@ static __device__ __forceinline__ void load_x(const T *row, uint32_t k, uint32_t
     }
 }
 
+// a lane's part of a 128-column chunk of a row of x: columns 32 s + 8 g .. + 7 for s = 0 .. 3.  A chunk that ends within the row is loaded whole before
+// anything is made of it (one after the other, each behind its own condition, they cost a round trip to memory each).
+template <typename T>
+static __device__ __forceinline__ void load_chunk(const T *row, uint32_t c, uint32_t g, uint32_t K, bool vec, bf16x8 out[4][XPlanes<T>::N])
+{
+    const uint32_t k = 128 * c + 8 * g;
+    if (vec && 128 * (c + 1) <= K) {
+        if constexpr (std::is_same<T, float>::value) {
+            f32x4 v[4][2];
+#pragma unroll
+            for (int s = 0; s < 4; s++) { v[s][0] = *(const f32x4 *)(row + k + 32 * s); v[s][1] = *(const f32x4 *)(row + k + 32 * s + 4); }
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const float y[8] = {v[s][0][0], v[s][0][1], v[s][0][2], v[s][0][3], v[s][1][0], v[s][1][1], v[s][1][2], v[s][1][3]};
+                Planes p;
+                split8(y, p);
+#pragma unroll
+                for (int i = 0; i < 3; i++) out[s][i] = p.p[i];
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; s++) out[s][0] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(row + k + 32 * s));
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < 4; s++) load_x<T>(row, k + 32 * s, K, vec, out[s]);
+    }
+}
+
 // eight e2m1 codes -> bf16 (exact)
 static __device__ __forceinline__ bf16x8 codes8(uint32_t w)
 {
@@ -97,6 +126,10 @@ __global__ __launch_bounds__(64 * W) void k_w4_linear_long(const T *x, uint64_t 
 #pragma unroll
             for (int q = 0; q < GROUPS; q++) sc[n][q] = *(const u32x2 *)(scales + ((t * chunks + c) * GROUPS + q) * 16 + 4 * g);
         }
+        // (four tiles and the planes of a whole chunk of fp32 would cost waves: 64 x 5000 x 1800 15.5 us, 13.5 with a quarter of the chunk at a time)
+        constexpr bool WHOLE = NT == 1 || XP == 1;
+        bf16x8 b[WHOLE ? 4 : 1][XP];
+        if constexpr (WHOLE) load_chunk<T>(xr, c, g, K, vec, b);
 #pragma unroll
         for (int q = 0; q < GROUPS; q++) {
             f32x4 d[NT];
@@ -104,13 +137,12 @@ __global__ __launch_bounds__(64 * W) void k_w4_linear_long(const T *x, uint64_t 
             for (int n = 0; n < NT; n++) d[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = q * GS; s < (q + 1) * GS; s++) {
-                bf16x8 b[XP];
-                load_x<T>(xr, 128 * c + 32 * s + 8 * g, K, vec, b);
+                if constexpr (!WHOLE) load_x<T>(xr, 128 * c + 32 * s + 8 * g, K, vec, b[0]);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     const bf16x8 a = codes8(w[n][s]);
 #pragma unroll
-                    for (int p = 0; p < XP; p++) d[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[p], d[n], 0, 0, 0);
+                    for (int p = 0; p < XP; p++) d[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[WHOLE ? s : 0][p], d[n], 0, 0, 0);
                 }
             }
 #pragma unroll
@@ -132,7 +164,7 @@ __global__ __launch_bounds__(64 * W) void k_w4_linear_long(const T *x, uint64_t 
 // At most 1024 columns: `kw` of a workgroup's eight waves (1, 2, 4 or 8) have one 128-column chunk each, 8 / kw such teams NT tiles of 16 outputs x MT tiles of 16 rows of
 // x.  A wave's chunk of x stays in its registers as planes (splitting fp32 into them costs more instructions than the products) while the workgroup goes
 // from tiles to tiles, every gridDim.x * 8 / kw * NT; the next round's codes are on their way while it works on these.  The waves' sums of two rounds lie side by side in LDS:
-// one barrier a round.  1 x 50265 x 1024 fp32 in 11.0 us, 2.5 TB/s of codes and scales; a launch and the first loads are 4 of them.
+// one barrier a round.  1 x 50265 x 1024 fp32 in 10.6 us, 2.6 TB/s of codes and scales; a launch and the first loads are 4 of them.
 template <typename T, int NT, int MT, int GS>
 __global__ __launch_bounds__(512, 2) void k_w4_linear_many(const T *x, uint64_t x_stride, const uint32_t *codes, const uint16_t *scales, const T *bias,
                                                            uint32_t M, uint32_t N, uint32_t K, uint32_t kw, uint32_t vec, uint32_t gelu, T *y)
@@ -156,11 +188,9 @@ __global__ __launch_bounds__(512, 2) void k_w4_linear_many(const T *x, uint64_t 
         }
     };
     fetch(mine);
-    bf16x8 b[4][MT][XP];
+    bf16x8 b[MT][4][XP];
 #pragma unroll
-    for (int s = 0; s < 4; s++)
-#pragma unroll
-        for (int m = 0; m < MT; m++) load_x<T>(x + (uint64_t)min(m0 + 16 * m + col, M - 1) * x_stride, 128 * cc + 32 * s + 8 * g, K, vec, b[s][m]);
+    for (int m = 0; m < MT; m++) load_chunk<T>(x + (uint64_t)min(m0 + 16 * m + col, M - 1) * x_stride, cc, g, K, vec, b[m]);
     uint32_t side = 0;
     for (uint32_t from = first; from < tiles; from += step, side ^= 1) {
         f32x4 acc[NT][MT];
@@ -191,7 +221,7 @@ __global__ __launch_bounds__(512, 2) void k_w4_linear_many(const T *x, uint64_t 
 #pragma unroll
                         for (int p = 0; p < XP; p++)
 #pragma unroll
-                            for (int m = 0; m < MT; m++) d[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[s][m][p], d[n][m], 0, 0, 0);
+                            for (int m = 0; m < MT; m++) d[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[m][s][p], d[n][m], 0, 0, 0);
                     }
 #pragma unroll
                 for (int n = 0; n < NT; n++)
@@ -267,11 +297,11 @@ static int w4_linear(void *stream, const void *x, uint64_t x_stride, const void 
     const uint32_t tiles = (N + 15) / 16, chunks = (K + 127) / 128;
     const W4Call c = {x, codes, scales, bias, y, x_stride, M, N, K, group, vec, gelu, chunks > 4 ? 8u : chunks > 2 ? 4u : chunks};
     // Measured (us; M x N x K):
-    //   x in registers against read again for each tile of outputs: 1 x 50265 x 1024 11.0 / 14.5, 64 x 50265 x 1024 fp32 33 / 63, 1 x 1024 x 1024 3.7 / 4.0.
+    //   x in registers against read again for each tile of outputs: 1 x 50265 x 1024 10.6 / 14.5, 64 x 50265 x 1024 fp32 33 / 63, 1 x 1024 x 1024 3.7 / 4.0.
     //   one tile a wave / two, where every CU has one anyway or not: 1 x 1024 x 1024 3.7 / 4.4, 4 x 4096 x 1024 3.9 / 4.2; 1 x 16384 x 1024 6.0 / 5.8,
     //   32 x 3000 x 1024 7.4 / 5.9, 64 x 50265 x 1024 36 / 33; four: 1 x 50265 x 1024 15.5.
     //   16 rows of x a wave / 32: fp32, whose planes take three times the registers, 64 x 50265 x 1024 33 / 37; bf16 27 / 24, 60 x 4096 x 1024 6.7 / 5.8, but 60 x 1024 x 1024 3.8 / 5.5.
-    //   more than 1024 columns, one tile / four: 1 x 1024 x 4096 6.2 / 11.8, 4 x 4096 x 2048 5.0 / 7.4; 40 x 24000 x 2000 bf16 32.9 / 23.1, 64 x 12000 x 4096 fp32 95 / 38.
+    //   more than 1024 columns, one tile / four: 1 x 1024 x 4096 6.2 / 11.8, 4 x 4096 x 2048 5.0 / 7.4; 40 x 24000 x 2000 bf16 33 / 20, 64 x 12000 x 4096 fp32 95 / 38.
     //   (32 rows a wave there: 50 to 97.)
     const uint64_t tiles16 = (uint64_t)tiles * ((M + 15) / 16), tiles32 = (uint64_t)tiles * ((M + 31) / 32);
     if (chunks <= 8) {
