@@ -802,12 +802,19 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void k_sample_tokens(Sample
                 const float x_at = __shfl(v, from);
                 const uint64_t incl = wave_scan(__shfl(in ? (uint64_t)w : 0, from)), left = wave_total(incl);
                 const double lse = row_lse();
-                for (uint32_t d = 0; d < a.draws; d++) {
-                    const uint64_t target = target_of(a.u[(uint64_t)row * a.draws + d], left), hit = __ballot(incl > target);
-                    if (lane + 1 == (uint32_t)__ffsll((unsigned long long)hit)) {
-                        a.tokens[(uint64_t)row * a.draws + d] = idx;
-                        a.logprobs[(uint64_t)row * a.draws + d] = (float)((double)x_at - lse);
+                for (uint32_t d0 = 0; d0 < a.draws; d0 += 64) {  // a draw a lane; where each falls is the wave's question
+                    const uint32_t many = min(a.draws - d0, 64u);
+                    const uint64_t at = (uint64_t)row * a.draws + d0 + lane, mine = target_of(lane < many ? a.u[at] : 0.f, left);
+                    int drawn = 0;
+                    for (uint32_t j = 0; j < many; j++) {
+                        const uint64_t target = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), (int)j) << 32) |
+                                                (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, (int)j);
+                        const int first = __ffsll((unsigned long long)__ballot(incl > target)) - 1;
+                        if (lane == j) drawn = first;
                     }
+                    const uint32_t token = __shfl(idx, drawn);
+                    const float x_drawn = __shfl(x_at, drawn);
+                    if (lane < many) { a.tokens[at] = token; a.logprobs[at] = (float)((double)x_drawn - lse); }
                 }
             }
         }

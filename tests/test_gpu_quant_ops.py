@@ -476,6 +476,15 @@ def test_sample_settings_row_by_row_and_strides():
     assert sample_tokens(wide[:, :V], torch.zeros(R, 0, device=DEV))[0].shape == (R, 0)
 
 
+@pytest.mark.parametrize("draws", [63, 64, 65, 1500])
+def test_sample_many_draws(draws):
+    """more draws than a wave has lanes, than a workgroup has waves and threads; rows that one wave finishes and rows that need them all"""
+    g = torch.Generator().manual_seed(draws)
+    x, u = torch.randn(3, 700, generator=g) * 4, torch.rand(3, draws, generator=g)
+    for kw in (dict(top_k=6), dict(top_k=50, top_p=0.9), dict(min_p=0.2), dict(top_p=0.9), dict()):
+        _check_samples(x, u, **kw)
+
+
 def test_sample_follows_the_distribution():
     """an even grid of u is a stratified sample: a token's share of the draws is off its probability by less than one draw at each end"""
     x = torch.tensor([[0.0, 1.0, -1.0, 2.0, 0.5]])
