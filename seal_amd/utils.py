@@ -2,8 +2,28 @@
 state dicts -> the HF ``BartForConditionalGeneration`` the decoder reads; graph capture with python's garbage collector held off."""
 import contextlib
 import gc
+import threading
 
 import torch
+
+
+# (of the process: a capture is, as torch.cuda.graph demands, the only one under way, and the collector has one switch)
+_CAPTURE = threading.RLock()
+
+
+@contextlib.contextmanager
+def collector_held():
+    """No collection of cyclic garbage in this process, and no other thread in here, while the block runs: what is dead goes before, what dies meanwhile waits.  The collector
+    is left as it was."""
+    with _CAPTURE:
+        gc.collect()
+        was = gc.isenabled()
+        gc.disable()
+        try:
+            yield
+        finally:
+            if was:
+                gc.enable()
 
 
 @contextlib.contextmanager
@@ -12,16 +32,10 @@ def captured(graph, **kwargs):
     (``model._seal_step_decoder``), so a decoder that is no longer used, and the graphs that it holds, go when the cyclic collector runs -- after any
     allocation, also one made inside another graph's capture.  The destructor of a ``torch.cuda.CUDAGraph`` synchronises the device on ROCm, which
     a capture forbids; its error leaves a destructor, and that ends the process (seen: "Fatal Python error: Aborted ... Garbage-collecting" under
-    ``tree_hidden_graph``).  So what is dead goes before the capture begins, and the collector waits until it has ended."""
-    gc.collect()
-    was = gc.isenabled()
-    gc.disable()
-    try:
-        with torch.cuda.graph(graph, **kwargs):
-            yield
-    finally:
-        if was:
-            gc.enable()
+    ``tree_hidden_graph``).  So what is dead goes before the capture begins, and the collector waits until it has ended.  Captures of several threads
+    take turns: the first to end would switch the collector on under the others."""
+    with collector_held(), torch.cuda.graph(graph, **kwargs):
+        yield
 
 
 _DERIVED_KEYS = {"lm_head.weight", "final_logits_bias", "model.encoder.embed_tokens.weight", "model.decoder.embed_tokens.weight",

@@ -1,0 +1,91 @@
+"""Captures of two threads at once (``seal_amd.utils.captured``): the collector is one switch for the process, so the thread that ends first must not switch it on under
+the other's capture, nor collect while the other captures.  On the CPU: the capture itself is replaced by a stand-in."""
+import contextlib
+import gc
+import threading
+
+import pytest
+import torch
+
+from seal_amd import utils
+
+
+@contextlib.contextmanager
+def _no_capture(graph, **kw):
+    yield
+
+
+@pytest.fixture(autouse=True)
+def stand_in(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "graph", _no_capture)
+    assert gc.isenabled()
+    yield
+    gc.enable()
+
+
+def test_a_capture_that_ends_leaves_the_collector_off_under_another():
+    seen, inside, go_on = [], threading.Event(), threading.Event()
+
+    def first():
+        with utils.captured(object()):
+            inside.set()
+            go_on.wait(10)
+
+    def second():
+        inside.wait(10)
+        with utils.captured(object()):               # (begins while the first is captured, or after it)
+            seen.append(gc.isenabled())
+            threads[0].join(0.5)                     # the first ends, if it has not yet
+            seen.append(gc.isenabled())
+    threads = [threading.Thread(target=first), threading.Thread(target=second)]
+    for t in threads:
+        t.start()
+    inside.wait(10)
+    threads[1].join(0.2)                             # (the second is inside by now, or waits)
+    go_on.set()
+    for t in threads:
+        t.join(20)
+        assert not t.is_alive()
+    assert seen == [False, False]
+    assert gc.isenabled()
+
+
+def test_no_thread_collects_for_its_own_capture_under_another():
+    calls, inside, go_on = [], threading.Event(), threading.Event()
+    capturing = []
+
+    def collect(*a):
+        calls.append(bool(capturing))
+        return 0
+
+    def first():
+        with utils.captured(object()):
+            capturing.append(1)
+            inside.set()
+            go_on.wait(10)
+            capturing.clear()
+
+    def second():
+        with utils.captured(object()):
+            pass
+    real, gc.collect = gc.collect, collect
+    try:
+        a, b = threading.Thread(target=first), threading.Thread(target=second)
+        a.start()
+        inside.wait(10)
+        b.start()
+        b.join(0.2)
+        go_on.set()
+        a.join(20)
+        b.join(20)
+    finally:
+        gc.collect = real
+    assert not a.is_alive() and not b.is_alive() and calls == [False, False]
+
+
+def test_a_capture_inside_a_held_block_of_the_same_thread():
+    with utils.collector_held():
+        with utils.captured(object()):
+            assert not gc.isenabled()
+        assert not gc.isenabled()
+    assert gc.isenabled()
