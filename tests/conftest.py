@@ -30,6 +30,35 @@ def _has_gpu():
         return False
 
 
+@pytest.fixture(scope="session", autouse=True)
+def captures_hold_the_collector():
+    """a test that captures with ``torch.cuda.graph`` itself: no collection may fall into that either (a dead decoder of an earlier test takes its graphs with
+    it, and freeing a graph inside a capture ends the process; see seal_amd.utils.captured)"""
+    import torch
+
+    from seal_amd.utils import collector_held
+    plain = torch.cuda.graph
+
+    class HeldGraph(plain):
+        def __enter__(self):
+            self.held = collector_held()
+            self.held.__enter__()
+            try:
+                return super().__enter__()
+            except BaseException:
+                self.held.__exit__(None, None, None)
+                raise
+
+        def __exit__(self, *exc):
+            try:
+                return super().__exit__(*exc)
+            finally:
+                self.held.__exit__(None, None, None)
+    torch.cuda.graph = HeldGraph
+    yield
+    torch.cuda.graph = plain
+
+
 def pytest_collection_modifyitems(config, items):
     if _has_gpu():
         return
