@@ -10,6 +10,7 @@ forward (``keys.py``) stay what ``BartStepDecoder`` runs.
     fm_index_sample(model, index, input_ids, attention_mask, num_samples=15, decoder=decoder)
     fm_index_generate(model, index, input_ids, attention_mask, keep_history=True, decoder=decoder, ...)
 """
+from collections import OrderedDict
 from typing import Optional
 
 import torch
@@ -17,7 +18,7 @@ import torch.nn.functional as F
 
 from .bart_decoder import BartStepDecoder
 from .kv8 import KV8Cache
-from .utils import captured
+from .utils import captured, collector_held
 from .w4 import quantize_w4, w4_linear
 
 
@@ -26,6 +27,10 @@ class QuantStepDecoder(BartStepDecoder):
     The model must be fp32 or bf16, on the GPU, with a head_dim of 64 or 128."""
 
     shared_first_step = False          # (every row is drawn or ranked on its own from the first step on)
+
+    # What the shapes that were decoded keep between decodes (caches, graphs and their logits), the least recently used going first: 300 rows of 1024 positions are 7.5 GB
+    # of history at BART-large, 64 positions 0.5 GB, and a graph holds at least the segments of a memory pool of its own.  The shape in use always stays.
+    STATE_BYTES, MAX_STATES = 16 << 30, 32
 
     def __init__(self, model, weights: Optional[str] = "w4", group: int = 32, block: int = 16):
         super().__init__(model)
@@ -37,7 +42,7 @@ class QuantStepDecoder(BartStepDecoder):
         if not w.is_cuda:
             raise RuntimeError("QuantStepDecoder: the model must live on the GPU (seal_amd has no CPU path)")
         self.block, self.quantized = block, weights is not None
-        self._states, self._cur = {}, None
+        self._states, self._cur = OrderedDict(), None
         self._w4 = {}
         if self.quantized:
             for L in self.layers:
@@ -54,7 +59,7 @@ class QuantStepDecoder(BartStepDecoder):
     class _State:
         pass
 
-    def _new_state(self, B, K, S, T, dtype, dev):
+    def _new_state(self, B, K, S, T, dev):
         st = self._State()
         R = B * K
         st.B, st.K = B, K
@@ -67,6 +72,30 @@ class QuantStepDecoder(BartStepDecoder):
         st.keep = torch.zeros(B, st.cross[0].tokens, dtype=torch.uint8, device=dev)
         st.dropped, st.graph, st.logits, st.tails = 0, None, None, {}
         return st
+
+    def _state_bytes(self, key, tails=()) -> int:
+        """what a shape holds: its caches, and the logits of its graphs (of all rows, and of the queries behind each of ``tails``)"""
+        B, K, S, T = key[:4]
+        codes = 2 * len(self.layers) * self.h * (B * K * T + B * S)
+        return codes * self.dh + codes // self.block * 4 + 4 * self.lm_w.shape[0] * K * (B + sum(B - dropped for dropped in tails))
+
+    def _make_room(self, key, dev) -> None:
+        """drop the least recently used shapes that ``key``'s leaves no room for"""
+        held = {k: self._state_bytes(k, st.tails) for k, st in self._states.items()}
+        held.setdefault(key, self._state_bytes(key))
+        total, drop = sum(held.values()), []
+        for k in self._states:                       # (the longest unused first)
+            if len(held) - len(drop) <= self.MAX_STATES and total <= self.STATE_BYTES:
+                break
+            if k != key:
+                drop.append(k)
+                total -= held[k]
+        if drop:
+            with collector_held():                   # (no graph may be freed under another thread's capture)
+                if dev.type == "cuda":
+                    torch.cuda.synchronize(dev)      # (a decode on another stream may still use what goes)
+                for k in drop:
+                    del self._states[k]
 
     @staticmethod
     def _tail(root, dropped):
@@ -138,10 +167,13 @@ class QuantStepDecoder(BartStepDecoder):
         self.batch, self.beams, self.rows, self.max_len, self.t = B, num_beams, B * num_beams, max_len, 0
         S64, T64 = -(-S // 64) * 64, -(-max_len // 64) * 64
         key = (B, num_beams, S64, T64, enc_hidden.dtype, str(dev))
+        self._root = self._cur = None                # (the last decode is over: its shape may go)
+        self._make_room(key, dev)
         st = self._states.get(key)
         if st is None:
             with torch.inference_mode(False):
-                st = self._states[key] = self._new_state(B, num_beams, S64, T64, enc_hidden.dtype, dev)
+                st = self._states[key] = self._new_state(B, num_beams, S64, T64, dev)
+        self._states.move_to_end(key)
         for dropped in narrow_plan:
             if dropped not in st.tails:
                 st.tails[dropped] = self._tail(st, dropped)

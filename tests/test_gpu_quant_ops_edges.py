@@ -1,0 +1,41 @@
+"""The quantised, sampled decode's operators at the edges of what their documentation allows, against the definitions in 64 bits (tests/quant_refs.py) or against the same
+call made the ordinary way."""
+import numpy as np
+import pytest
+import torch
+
+from tests import quant_refs as ref
+from tests import test_gpu_quant_ops as ops
+from tests.helpers import tiny_bart
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+# ---------------------------------------------------------------------------
+# what a decoder keeps
+# ---------------------------------------------------------------------------
+def test_a_decoder_that_forgets_shapes_decodes_the_same():
+    """more shapes than are kept: each decode equals that of a decoder which has seen no other, also one whose shape went and came back"""
+    from seal_amd.quant_decoder import QuantStepDecoder
+    model = tiny_bart(130, d_model=128, heads=2, max_positions=160).to(DEV)
+    g = torch.Generator().manual_seed(17)
+    dec = QuantStepDecoder(model)
+    dec.MAX_STATES = 2
+
+    def decode(d, B, S, T, plan=()):
+        ids, mask, toks = inputs[B, S, T]
+        d.start(d.encode(ids, mask), mask, 2, T, narrow_plan=plan)
+        return [d.step(t).clone() for t in toks]
+    inputs = {}
+    shapes = [(1, 10, 8), (2, 70, 8), (3, 10, 70), (2, 10, 8)]
+    for B, S, T in shapes:
+        ids = torch.randint(4, 122, (B, S), generator=g).to(DEV)
+        inputs[B, S, T] = ids, torch.ones_like(ids), [torch.randint(4, 122, (2 * B,), generator=g).to(DEV) for _ in range(6)]
+    first = [decode(QuantStepDecoder(model), *s) for s in shapes]
+    for _ in range(2):
+        for s, want in zip(shapes, first):
+            got = decode(dec, *s, plan=(1,) if s[0] > 1 else ())
+            assert len(dec._states) <= 2
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
