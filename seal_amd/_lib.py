@@ -238,6 +238,13 @@ def launch(fn, index: int, *args) -> None:
         check(rc)
 
 
+def refuse_gradient(who: str, *tensors) -> None:
+    """an error, where a result without history would lose a gradient silently"""
+    import torch
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{who} has no backward pass, and an input requires a gradient: call it under torch.no_grad(), or detach the input")
+
+
 def check(rc: int) -> None:
     if rc != 0:
         raise SealFMError(rc, lib().fmi_last_error().decode("utf-8", "replace"))

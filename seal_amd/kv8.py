@@ -8,7 +8,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import launch, lib, uint64s
+from ._lib import launch, lib, refuse_gradient, uint64s
 
 TILE = 64                                  # tokens of a tile of the layout
 # Workgroups (of four waves) that a call splits long slots into when it has few: one a CU is enough for many items (32 slots x 8 heads of up to 8192 tokens: 79 us, in two
@@ -20,7 +20,8 @@ ITEMS_ENOUGH, PARTS_WANTED, SPLIT_TOKENS = 256, 512, 1024
 class KV8Cache:
     """``k`` [slots, heads, T, head_dim] and ``v`` [slots, heads, T / 64, head_dim, 64] uint8 (e4m3 codes; token 16 j + 4 g + r of a tile at place
     16 g + 4 j + r), ``k_scale`` / ``v_scale`` [slots, heads, T / block] fp32 powers of two.  T a multiple of 64, head_dim 64 or 128, block 16, 32 or 64.
-    ``KV8Cache.empty`` makes the buffers."""
+    ``KV8Cache.empty`` makes the buffers.  For serving: ``append`` and ``attend`` have no gradient, and refuse inputs that require one unless called under
+    ``torch.no_grad()``."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         shape, blocks = k.shape, k_scale.shape
@@ -74,6 +75,8 @@ class KV8Cache:
         ks, vs = k_new.stride(), v_new.stride()
         if ks[3] != 1 or vs[3] != 1:
             raise ValueError("KV8Cache.append: the dims of a head must be contiguous")
+        if k_new.requires_grad or v_new.requires_grad:
+            refuse_gradient("KV8Cache.append", k_new, v_new)
         lengths_ptr, counts_ptr = self._lengths(lengths, "lengths"), None if counts is None else self._lengths(counts, "counts")
         launch(lib().sealnn_kv8_append if dt == torch.float32 else lib().sealnn_kv8_append_bf16, self._on_gpu(), k_new.data_ptr(), v_new.data_ptr(),
                uint64s(ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), shape[1], lengths_ptr, counts_ptr, self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
@@ -92,6 +95,8 @@ class KV8Cache:
         row_stride, head_stride, stride = q.stride()
         if stride != 1:
             raise ValueError("KV8Cache.attend: the dims of a head must be contiguous")
+        if q.requires_grad:
+            refuse_gradient("KV8Cache.attend", q)
         share = shape[1] // H
         keep_ptr, keep_stride = None, 0
         if keep is not None:

@@ -7,7 +7,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from ._lib import launch, lib
+from ._lib import launch, lib, refuse_gradient
 
 MAX_VOCAB = 1 << 18
 # Few rows of a large vocabulary are spread over the card by three kernels instead of one workgroup each (include/sealnn.h).  us, one kernel / three, fp32, top-p 0.9: 1 x 16384
@@ -38,7 +38,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     for all rows or a tensor with one for each row (fp32; ``top_k`` int32).  NaN logits are never drawn, +inf counts as the largest fp32 number.
 
     A row of which no token may be drawn gives token -1 and log-probability -inf.  ``logprobs`` are those of the model: ``logit - logsumexp`` of the whole
-    row, without temperature, constraint or filters (what the decode loop carries, as the reference's beam scores carry unconstrained ones)."""
+    row, without temperature, constraint or filters (what the decode loop carries, as the reference's beam scores carry unconstrained ones).  No gradient: logits that require one are refused unless it is
+    called under ``torch.no_grad()``."""
     dt, shape, dev, u_shape = logits.dtype, logits.shape, logits.device, u.shape
     if len(shape) != 2 or (dt != torch.float32 and dt != torch.bfloat16):
         raise ValueError(f"sample_tokens: logits are fp32 or bf16 [rows, vocab], got {dt} {tuple(shape)}")
@@ -52,6 +53,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
         raise ValueError("sample_tokens: the rows of the logits overlap")
     if u.dtype != torch.float32 or not 0 < len(u_shape) < 3 or u_shape[0] != rows or u.device != dev:
         raise ValueError(f"sample_tokens: u is fp32 [rows] or [rows, draws] on {dev}, got {u.dtype} {tuple(u_shape)} on {u.device}")
+    if logits.requires_grad:
+        refuse_gradient("sample_tokens", logits)
     u = u.contiguous()
     t = k = p = m = 0
     t_v = k_v = p_v = m_v = None

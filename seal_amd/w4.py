@@ -7,7 +7,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import launch, lib
+from ._lib import launch, lib, refuse_gradient
 
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -64,7 +64,7 @@ def quantize_w4(weight: torch.Tensor, group: int = 32) -> W4Weight:
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None, gelu: bool = False) -> torch.Tensor:
     """``F.linear(x, weight, bias)`` (and its erf GELU) for ``x`` fp32 or bf16 [rows, in_features], rows may be strided; ``bias`` of x's type.  Made for 1 .. 64 rows; up
-    to 2^19 work.  Returns a new [rows, out_features] of x's type."""
+    to 2^19 work.  Returns a new [rows, out_features] of x's type.  No gradient: an input that requires one is refused unless it is called under ``torch.no_grad()``."""
     codes, dt = weight.codes, x.dtype
     if x.dim() != 2 or x.shape[1] != weight.in_features or (dt != torch.float32 and dt != torch.bfloat16) or x.device != codes.device:
         raise ValueError(f"w4_linear: x is fp32 or bf16 [rows, {weight.in_features}] on {codes.device}, got {dt} {tuple(x.shape)} on {x.device}")
@@ -74,6 +74,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
         raise ValueError("w4_linear: the columns of a row of x must be contiguous")
     if bias is not None and (bias.shape != (N,) or bias.dtype != dt or bias.device != x.device or not bias.is_contiguous()):
         raise ValueError(f"w4_linear: the bias is {dt} [{N}], contiguous, on {x.device}")
+    if x.requires_grad or (bias is not None and bias.requires_grad):
+        refuse_gradient("w4_linear", x, bias)
     if not x.is_cuda:
         raise RuntimeError("w4_linear: x must live on the GPU (seal_amd has no CPU path)")
     y = x.new_empty((rows, N))

@@ -1,0 +1,37 @@
+"""What the quantised, sampled decode's Python entries refuse beyond shapes and types, and what quantising has to get right at the edge of a type's range.  No GPU."""
+import pytest
+import torch
+
+from seal_amd.kv8 import KV8Cache
+from seal_amd.sampling import sample_tokens
+from seal_amd.w4 import quantize_w4, w4_linear
+
+
+def _calls():
+    c, n = KV8Cache.empty(2, 1, 64, 64, device="cpu"), torch.zeros(2, dtype=torch.int32)
+    kv, w = torch.zeros(2, 1, 1, 64), quantize_w4(torch.randn(16, 128))
+    return {
+        "sample_tokens": (lambda t: sample_tokens(t, torch.zeros(2)), torch.zeros(2, 70)),
+        "w4_linear": (lambda t: w4_linear(t, w), torch.zeros(2, 128)),
+        "w4_linear bias": (lambda t: w4_linear(torch.zeros(2, 128), w, t), torch.zeros(16)),
+        "KV8Cache.append keys": (lambda t: c.append(t, kv, n), kv.clone()),
+        "KV8Cache.append values": (lambda t: c.append(kv, t, n), kv.clone()),
+        "KV8Cache.attend": (lambda t: c.attend(t, n), torch.zeros(2, 1, 64)),
+    }
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+def test_a_gradient_is_refused_not_lost(name):
+    call, t = _calls()[name]
+    t.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="backward"):
+        call(t)
+    with pytest.raises(RuntimeError, match="backward"):
+        call(t * 2)                                       # (a result with history)
+    # without a gradient to lose the call goes on, here as far as the missing GPU
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+        call(t)
+    with torch.inference_mode(), pytest.raises(RuntimeError, match="GPU"):
+        call(t)
+    with pytest.raises(RuntimeError, match="GPU"):
+        call(t.detach())
