@@ -128,6 +128,8 @@ class KV8Cache:
         return scaled(self.k, self.k_scale), scaled(v, self.v_scale)
 
     def reorder(self, rows: torch.Tensor) -> None:
-        """slot i continues what slot ``rows[i]`` held (HF ``_reorder_cache``)"""
+        """slot i continues what slot ``rows[i]`` held (HF ``_reorder_cache``); ``rows`` int64 or int32 [slots], on the device, each 0 .. slots - 1"""
+        if rows.shape != (self.slots,) or rows.dtype not in (torch.int64, torch.int32) or rows.device != self.device:
+            raise ValueError(f"KV8Cache.reorder: rows are int64 or int32 [{self.slots}] on {self.device}, got {rows.dtype} {tuple(rows.shape)} on {rows.device}")
         for t in (self.k, self.v, self.k_scale, self.v_scale):
             t.copy_(t.index_select(0, rows))

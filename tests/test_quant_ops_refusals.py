@@ -35,3 +35,21 @@ def test_a_gradient_is_refused_not_lost(name):
         call(t)
     with pytest.raises(RuntimeError, match="GPU"):
         call(t.detach())
+
+
+def test_reorder_takes_a_row_for_every_slot():
+    """a single row would be copied into every slot"""
+    c = KV8Cache.empty(3, 2, 64, 64, device="cpu")
+    for t in (c.k, c.v):
+        t.copy_(torch.randint(0, 127, t.shape, dtype=torch.uint8))
+    for t in (c.k_scale, c.v_scale):
+        t.copy_(torch.exp2(torch.randint(-3, 3, t.shape).float()))
+    held = [t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale)]
+    for bad in (torch.tensor([1]), torch.tensor([0, 1]), torch.tensor([[0, 1, 2]]), torch.tensor([0.0, 1.0, 2.0]), torch.tensor([True, False, True]), torch.tensor(1)):
+        with pytest.raises(ValueError):
+            c.reorder(bad)
+        assert all(torch.equal(a, b) for a, b in zip((c.k, c.v, c.k_scale, c.v_scale), held))
+    for dt in (torch.int64, torch.int32):
+        c.reorder(torch.tensor([2, 2, 0], dtype=dt))
+        assert all(torch.equal(a, b[[2, 2, 0]]) for a, b in zip((c.k, c.v, c.k_scale, c.v_scale), held))
+        held = [t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale)]
