@@ -103,6 +103,8 @@ class KV8Cache:
             if keep.shape != (self.slots, self.tokens) or keep.dtype not in (torch.bool, torch.uint8) or keep.device != self.device:
                 raise ValueError(f"KV8Cache.attend: keep is bool or uint8 [{self.slots}, {self.tokens}] on {self.device}, got {keep.dtype} {tuple(keep.shape)}")
             keep = keep.contiguous()
+            if keep.data_ptr() & 3:                  # (the kernel reads four tokens' bytes as a word: a view that starts between words is copied)
+                keep = keep.clone()
             keep_ptr, keep_stride = keep.data_ptr(), self.tokens
         lengths_ptr, index = self._lengths(lengths, "lengths"), self._on_gpu()
         out = q.new_empty(shape)

@@ -39,3 +39,26 @@ def test_a_decoder_that_forgets_shapes_decodes_the_same():
             got = decode(dec, *s, plan=(1,) if s[0] > 1 else ())
             assert len(dec._states) <= 2
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------
+# the cache
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("T,beams", [(64, 1), (64, 3), (128, 2)])
+def test_a_mask_that_starts_between_words(T, beams):
+    """a contiguous view at any byte, and rows cut out of a wider mask"""
+    g = torch.Generator().manual_seed(T)
+    S, H, D = 3, 2, 64
+    c = ops._filled(S, H, T, D, 16, g)
+    q = torch.randn(S * beams, H, D, generator=g).to(DEV)
+    ln = torch.tensor([T, T - 7, 5], dtype=torch.int32, device=DEV)
+    keep = (torch.rand(S, T, generator=g) < 0.5).to(DEV)
+    want = c.attend(q, ln, beams=beams, keep=keep)
+    for off in (1, 2, 3, 4):
+        flat = torch.zeros(S * T + 4, dtype=torch.bool, device=DEV)
+        view = flat[off:off + S * T].view(S, T)
+        view.copy_(keep)
+        assert view.is_contiguous() and torch.equal(c.attend(q, ln, beams=beams, keep=view), want)
+    wide = torch.zeros(S, T + 5, dtype=torch.bool, device=DEV)
+    wide[:, 3:3 + T] = keep
+    assert torch.equal(c.attend(q, ln, beams=beams, keep=wide[:, 3:3 + T]), want)
