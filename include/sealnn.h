@@ -148,7 +148,9 @@ int sealnn_hgemm_nt_ep(void *stream, const void *a, const void *w, float *c, uin
  *   codes   [ceil(N / 16)][ceil(K / 128)][4 g][16 row][4 s][4] bytes: the four bytes hold the e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign)
  *           of columns 32 s + 8 g .. + 7 of row `row` of the 16 x 128 tile, the even column in the low nibble; columns from K on are zero
  *   scales  [ceil(N / 16)][ceil(K / 128) * 128 / group][16] bf16; group 32, 64 or 128 columns of a row
- * fp32 x is used to its last bit (three bf16 planes), sums are fp32.  A non-finite x makes its row's products NaN. */
+ * fp32 x is used to its last bit (three bf16 planes), sums are fp32; a group's columns are summed before their scale (finite for |x| <= 2^118).  A NaN in a row of x makes
+ * the row's outputs NaN, and so does an infinity in fp32 (its lower planes are inf - inf); an infinity in bf16 gives what inf * w sums to: +-inf, or NaN where
+ * a code of its column is 0 or two infinities cancel.  Other rows are not touched. */
 int sealnn_w4_linear(void *stream, const float *x, uint64_t x_stride, const void *codes, const void *scales, const float *bias, uint32_t M, uint32_t N,
                      uint32_t K, uint32_t group, uint32_t gelu, float *y);
 int sealnn_w4_linear_bf16(void *stream, const void *x, uint64_t x_stride, const void *codes, const void *scales, const void *bias, uint32_t M, uint32_t N,

@@ -62,3 +62,31 @@ def test_a_mask_that_starts_between_words(T, beams):
     wide = torch.zeros(S, T + 5, dtype=torch.bool, device=DEV)
     wide[:, 3:3 + T] = keep
     assert torch.equal(c.attend(q, ln, beams=beams, keep=wide[:, 3:3 + T]), want)
+
+
+# ---------------------------------------------------------------------------
+# products
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("K,N", [(256, 40), (1300, 40), (1300, 9000)])
+def test_a_row_that_is_not_finite(K, N):
+    """NaN: the whole row; an infinity: NaN in fp32, what inf * w sums to in bf16; the other rows stay"""
+    from seal_amd.w4 import quantize_w4, w4_linear
+    g = torch.Generator().manual_seed(K)
+    w = quantize_w4(torch.randn(N, K, generator=g).to(DEV), 32)
+    W = w.dequantize()
+    for dt in (F32, BF16):
+        x = torch.randn(20, K, generator=g).to(dt).to(DEV)
+        want = w4_linear(x, w)
+        x[3, 17], x[18, K - 1], x[19, 0], x[19, 5] = float("nan"), float("inf"), float("inf"), -float("inf")
+        got = w4_linear(x, w)
+        assert torch.equal(torch.cat([got[:3], got[4:18]]), torch.cat([want[:3], want[4:18]]))
+        assert torch.isnan(got[3]).all()
+        if dt == F32:
+            assert torch.isnan(got[18:]).all()
+        else:
+            col = W[:, K - 1]
+            assert torch.equal(torch.isnan(got[18]), col == 0)
+            assert torch.equal(got[18][col != 0].float(), torch.sign(col[col != 0]) * float("inf"))
+            a, b = torch.sign(W[:, 0]), -torch.sign(W[:, 5])
+            both = (a != 0) & (a == b)
+            assert torch.equal(torch.isnan(got[19]), ~both) and torch.equal(got[19][both].float(), a[both] * float("inf"))
