@@ -90,3 +90,99 @@ def test_a_row_that_is_not_finite(K, N):
             a, b = torch.sign(W[:, 0]), -torch.sign(W[:, 5])
             both = (a != 0) & (a == b)
             assert torch.equal(torch.isnan(got[19]), ~both) and torch.equal(got[19][both].float(), a[both] * float("inf"))
+
+
+def _tokens(v):
+    """the cache's V, token by token: [slots, heads, T, dh] (a copy)"""
+    S, H, n, D, _ = v.shape
+    return v.view(S, H, n, D, 4, 4, 4).permute(0, 1, 2, 5, 4, 6, 3).reshape(S, H, n * 64, D)
+
+
+def _tiles(v):
+    S, H, T, D = v.shape
+    return v.view(S, H, T // 64, 4, 4, 4, D).permute(0, 1, 2, 6, 4, 3, 5).reshape(S, H, T // 64, D, 64)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,share,beams", [(64, 1, 1), (64, 1, 15), (64, 4, 1), (64, 1, 17), (128, 1, 1), (128, 1, 15)])
+@pytest.mark.parametrize("block", [16, 64])
+def test_attend_among_garbage(T, share, beams, block, D, dt):
+    """caches as a decode that is not the first finds them, for every kernel of the attention: any codes, NaN among them, behind the lengths and under the mask, and scales that are NaN or
+    infinite where a block has no token that counts"""
+    g = torch.Generator().manual_seed(T + beams + share + block)
+    S, H = 6, 2
+    c = ops._filled(S, H, T, D, block, g, garbage=True)
+    lengths = [0, 1, 16, 17, T - 1, T]
+    keep = torch.rand(S, T, generator=g) < 0.6
+    keep[1, 0] = True
+    keep[4] = False                                       # nothing left
+    keep[5, 16:32] = False
+    live = keep & (torch.arange(T) < torch.tensor(lengths)[:, None])
+    at = live[:, None, :, None].to(DEV)
+    tame = lambda t: torch.where(at & ((t & 127) == 127), t - 1, t)  # noqa: E731
+    c.k.copy_(tame(c.k))
+    c.v.copy_(_tiles(tame(_tokens(c.v))))
+    dead = ~live.view(S, T // block, block).any(-1)[:, None].expand(S, H, T // block).to(DEV)
+    for t, bad in ((c.k_scale, float("nan")), (c.v_scale, float("inf"))):
+        t.masked_fill_(dead, bad)
+    assert bool(dead.any()) and bool(((c.k & 127) == 127).any()) and bool(((c.v & 127) == 127).any())
+    q = (torch.randn(S * beams, H * share, D, generator=g) * 0.3).to(dt)
+    k, v = ops._refs(c)
+    with np.errstate(invalid="ignore"):
+        kv, vv = k.values(), v.values()
+    want, mag, vmax = ref.attend(q.double().numpy(), kv, vv, lengths, beams, keep.numpy())
+    got = c.attend(q.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), beams=beams, keep=keep.to(DEV)).double().cpu().numpy()
+    assert (np.abs(got - want) <= ops._attend_bound(mag, T, want, D, vmax, dt)).all()
+    assert not got[:beams].any() and not got[4 * beams:5 * beams].any()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_nan_among_the_tokens_of_one_tile_shows(D, dt):
+    g = torch.Generator().manual_seed(5)
+    for beams in (1, 3):
+        c = ops._filled(3, 1, 64, D, 16, g)
+        q, ln = torch.randn(3 * beams, 1, D, generator=g).to(dt).to(DEV), torch.tensor([40, 40, 40], dtype=torch.int32, device=DEV)
+        want = c.attend(q, ln, beams=beams)
+        c.k[1, 0, 20, D - 1] = 0x7f
+        c.v[2, 0, 0, D - 1, ref.place(39)] = 0xff
+        got = c.attend(q, ln, beams=beams)
+        assert torch.equal(got[:beams], want[:beams]) and torch.isnan(got[beams:2 * beams]).all()
+        assert torch.isnan(got[2 * beams:, :, D - 1]).all() and torch.equal(got[2 * beams:, :, :D - 1], want[2 * beams:, :, :D - 1])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D,block", [(64, 16), (128, 16), (64, 64), (128, 32)])
+def test_append_of_one_token_with_counts_and_odd_values(D, block, dt):
+    """the single-token kernel: slots that bring none, values that are not finite, zeros, scales that grow, lengths outside the cache; step by step, all buffers compared each time"""
+    g = torch.Generator().manual_seed(D + block)
+    S, H, T = 6, 3, 64
+    c = ops._filled(S, H, T, D, block, g)
+    k, v = ops._refs(c)
+    lengths = torch.tensor([0, 14, 15, 30, 63, 7], dtype=torch.int32)
+    odd = [0.0, float("inf"), -float("inf"), float("nan"), 448.0, 449.0, 1e-30, 1e30]
+    for step in range(12):
+        x = (torch.randn(S, 1, 2, H, D, generator=g) * 2.0 ** (2 * step - 8))
+        counts = torch.randint(0, 2, (S,), generator=g).to(torch.int32)
+        for s in range(S):
+            for o in odd[step % 8:step % 8 + 3]:
+                x[s, 0, int(torch.randint(0, 2, (1,), generator=g)), int(torch.randint(0, H, (1,), generator=g)), int(torch.randint(0, D, (1,), generator=g))] = o
+        if step % 5 == 4:
+            x[:] = 0
+        if step == 6:
+            x[2] = float("nan")
+            x[3] = float("inf")
+            counts[2:4] = 1
+        if step == 9:
+            counts = torch.tensor([7, -1, 1, 0, 1, 2], dtype=torch.int32)     # (never more than the token that is there)
+        x = x.to(dt)
+        c.append(x.to(DEV)[:, :, 0], x.to(DEV)[:, :, 1], lengths.to(DEV), None if step == 3 else counts.to(DEV))
+        brought = torch.ones_like(counts) if step == 3 else counts.clamp(0, 1)
+        k.append(x[:, :, 0].double().numpy(), lengths.tolist(), brought.tolist())
+        v.append(x[:, :, 1].double().numpy(), lengths.tolist(), brought.tolist())
+        ops._assert_same(c, k, v)
+        lengths += brought
+        lengths[4] = 63 if step % 2 else 64                # (full: dropped)
+        if step == 7:
+            lengths[0] = -1
