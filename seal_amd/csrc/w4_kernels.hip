@@ -304,12 +304,14 @@ static int w4_linear(void *stream, const void *x, uint64_t x_stride, const void 
     //   more than 1024 columns, one tile / four: 1 x 1024 x 4096 6.2 / 11.8, 4 x 4096 x 2048 5.0 / 7.4; 40 x 24000 x 2000 bf16 33 / 20, 64 x 12000 x 4096 fp32 95 / 38.
     //   (32 rows a wave there: 50 to 97.)
     const uint64_t tiles16 = (uint64_t)tiles * ((M + 15) / 16), tiles32 = (uint64_t)tiles * ((M + 31) / 32);
-    if (chunks <= 8) {
-        if (std::is_same<T, bf16>::value && M > 16 && tiles32 >= 512) launch_many<T, 2, 2>(st, c);
-        else if (tiles16 > 256) launch_many<T, 2, 1>(st, c);
-        else launch_many<T, 1, 1>(st, c);
-    } else if (tiles16 >= 1024) launch_long<T, 4, 8>(st, c);
-    else launch_long<T, 1, 16>(st, c);
+    auto rows16 = [&] { if (tiles16 > 256) launch_many<T, 2, 1>(st, c); else launch_many<T, 1, 1>(st, c); };
+    if (chunks > 8) {
+        if (tiles16 >= 1024) launch_long<T, 4, 8>(st, c);
+        else launch_long<T, 1, 16>(st, c);
+    } else if constexpr (std::is_same<T, bf16>::value) {
+        if (M > 16 && tiles32 >= 512) launch_many<T, 2, 2>(st, c);
+        else rows16();
+    } else rows16();
     NNCHK();
     return FMI_OK;
 }
