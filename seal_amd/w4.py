@@ -42,15 +42,15 @@ def quantize_w4(weight: torch.Tensor, group: int = 32) -> W4Weight:
     code with the even last bit.  Any device."""
     if weight.dim() != 2 or group not in (32, 64, 128):
         raise ValueError(f"quantize_w4: a weight [out, in] and a group of 32, 64 or 128, got {tuple(weight.shape)} and {group}")
-    if not bool(torch.isfinite(weight).all()):
-        raise ValueError("quantize_w4: the weight holds infinities or NaN")
     N, K = weight.shape
     Np, Kp = -(-N // 16) * 16, -(-K // 128) * 128
     w = torch.zeros(Np, Kp, dtype=torch.float32, device=weight.device)
     w[:N, :K] = weight
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("quantize_w4: the weight holds infinities or NaN, or numbers beyond fp32")
     g = w.view(Np, Kp // group, group)
     s = (g.abs().amax(-1) / 6).to(torch.bfloat16)
-    y = (g / s.float().clamp_min(torch.finfo(torch.float32).tiny).unsqueeze(-1)).view(Np, Kp)
+    y = (g / torch.where(s > 0, s, 1.0).float().unsqueeze(-1)).view(Np, Kp)      # (a scale of 0: every multiple is 0)
     mag = y.abs()
     lut = torch.tensor(E2M1, device=w.device)
     mid = (lut[1:] + lut[:-1]) / 2

@@ -186,3 +186,18 @@ def test_append_of_one_token_with_counts_and_odd_values(D, block, dt):
         lengths[4] = 63 if step % 2 else 64                # (full: dropped)
         if step == 7:
             lengths[0] = -1
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-36, 1e-38, 3e-39, 1e-40])
+def test_weights_are_quantised_alike_on_the_gpu_and_multiply_with_tiny_scales(size):
+    """scales below the smallest normal number: the same codes as on the CPU, and the product still applies them (fp32 has them as subnormals; x large enough that y is normal)"""
+    from seal_amd.w4 import quantize_w4, w4_linear
+    g = torch.Generator().manual_seed(8)
+    w = (torch.rand(33, 300, generator=g) * 2 - 1) * size
+    a, b = quantize_w4(w, 32), quantize_w4(w.to(DEV), 32)
+    assert torch.equal(a.codes, b.codes.cpu()) and torch.equal(a.scales, b.scales.cpu())
+    x = torch.randn(3, 300, generator=g) * (1 / size if size > 1e-38 else 1e36)
+    W, X = a.dequantize().double().numpy(), x.double().numpy()
+    want = X @ W.T
+    got = w4_linear(x.to(DEV), b).double().cpu().numpy()
+    assert (np.abs(got - want) <= ops._product_bound(X, W, want, 300, F32)).all()

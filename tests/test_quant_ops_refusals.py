@@ -53,3 +53,26 @@ def test_reorder_takes_a_row_for_every_slot():
         c.reorder(torch.tensor([2, 2, 0], dtype=dt))
         assert all(torch.equal(a, b[[2, 2, 0]]) for a, b in zip((c.k, c.v, c.k_scale, c.v_scale), held))
         held = [t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale)]
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("size", [1e-36, 1e-38, 3e-39, 1e-40, 3e-41, 1e-44, 3e38])
+def test_tiny_and_huge_weights_are_the_nearest_multiples_too(size, group):
+    """scales below the smallest normal number (bf16 has fp32's subnormals, with 8 bits less), scales that round to zero, weights up to the largest number"""
+    from tests import quant_refs as ref
+    g = torch.Generator().manual_seed(3)
+    w = (torch.rand(20, 300, generator=g) * 2 - 1) * size
+    w[0, :40] = 0
+    q = quantize_w4(w, group)
+    got = ref.w4_values(q.codes.numpy(), q.scales.float().numpy(), 20, 300)
+    s = q.scales.double().transpose(1, 2).reshape(-1, q.scales.shape[1]).numpy().repeat(group, 1)[:20, :300]
+    best = abs(ref.E2M1[:, None, None] * s - w.double().numpy()).min(0)
+    assert (abs(got - w.double().numpy()) == best).all()
+    assert torch.equal(q.dequantize().double(), torch.from_numpy(got))
+
+
+def test_weights_beyond_fp32_are_refused():
+    w = torch.zeros(4, 64, dtype=torch.float64)
+    w[1, 2] = 1e300
+    with pytest.raises(ValueError):
+        quantize_w4(w)
