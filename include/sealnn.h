@@ -186,6 +186,7 @@ int sealnn_kv8_attend_bf16(void *stream, const void *q, uint64_t q_row_stride, u
  *   are among the top_k largest (0: off; equal logits: the lower index first), then
  *   among the fewest largest of those that hold at least top_p of their weight (>= 1: off), and
  *   have at least min_p of the largest weight (<= 0: off).
+ * A weight is a whole multiple of 2^-44 of the largest's (off by half of that and by 2^-39 of itself): one below 2^-45 is 0, and its token is never drawn.
  * temperature <= 0: the first of the largest.  The *_v arrays ([rows], or NULL) override the numbers row by row.  NaN logits are never drawn, +inf counts as the
  * largest fp32 number.  tokens / logprobs [rows][draws]: -1 / -inf for a row without a token; logprobs = logit - logsumexp(row), neither
  * temperature nor filters applied.

@@ -325,8 +325,9 @@ __global__ __launch_bounds__(256) void k_kv8_append(AppendArgs a, uint32_t vec)
 // Both operands come from memory straight into the registers that the instruction reads: the contraction index of a matrix instruction may be
 // permuted as long as both operands agree, so lane (g, t) takes 16 consecutive bytes of token t of K (dims 16 g .. of a 64-dim half), and the
 // S values that a lane holds (tokens 16 j + 4 g + r of its query) are, unmoved, the B operand of the second product -- V's tiles are laid out
-// for that.  q and p are fp32 numbers and enter as three bf16 planes each (exact); for bf16 queries q is one plane and p two (2^-17 relative:
-// the rounding of p stays far below the output's own).  A block's scale is a factor of S's rows (K) or of p (V).
+// for that.  q and p are fp32 numbers and enter as three bf16 planes each (exact); for bf16 queries q is one plane and p two
+// (what they leave of p is cut off: up to 2^-15 of it, about 2^-17 on average, always towards zero while the sum l takes p whole; the store's own half step is 2^-8).
+// A block's scale is a factor of S's rows (K) or of p (V).
 // Bytes behind `length` or masked may be anything: S is selected, p is 0 there and V's bytes are cleared.
 // Measured: 32 slots x 8 heads of 4001 .. 8192 tokens, dh 128, bf16 80 us, 5.0 TB/s (memory); 1 slot x 16 heads of 32001 tokens bf16 in 32 parts 18.3 us, 3.6 TB/s, the join
 // 3 of them; 40 slots x 16 heads x 15 beams of 500 .. 1024 tokens fp32 20.6 us, 3.3 TB/s (640 workgroups on 256 CUs, and the planes' arithmetic); 20 x 16 heads x 15

@@ -6,8 +6,9 @@
 // by counting (or weighing) buckets of logits and looking again inside the one bucket that the border falls into, and then draws in the order
 // of the vocabulary from the tokens above it: the first token whose cumulative weight passes u * total.
 //
-// Weights are whole numbers, exp((x - max) / T) * 2^44 to nearest, computed in 64-bit floats and added in 64-bit integers: sums of up to 2^18 of
-// them are exact, so neither the order of the atomics nor the shape of a reduction changes which token a random number falls on.
+// Weights are whole numbers, exp((x - max) / T) * 2^44 rounded, computed in 64-bit floats (the exponential to 2^-39 of itself: up to 21 units near the
+// largest, less than the rounding's half unit below 2^-6 of it) and added in 64-bit integers: sums of up to 2^18 of them are exact, so neither the order of the atomics nor the shape of a reduction changes which
+// token a random number falls on.  A weight below 2^-45 of the largest is 0.
 #include "nn_common.h"
 
 #include <algorithm>
@@ -67,8 +68,8 @@ struct Shared {
     uint64_t before, total;
 };
 
-// exp((x - m) / T) * 2^44 to nearest, as a 64-bit float (a whole number; 0 below 2^-45): 2^t = 2^floor * 2^(k / 32) * e^y, |y| <= ln 2 / 64, where the
-// series ends at y^4 (y^5 / 120 < 2^-39 relative, below the step of any weight that is not near the largest)
+// exp((x - m) / T) * 2^44 as a 64-bit float (a whole number; 0 below 2^-45): 2^t = 2^floor * 2^(k / 32) * e^y, |y| <= ln 2 / 64, where the
+// series ends at y^4 (what it leaves out is y^5 / 120 < 2^-39 relative: below half a unit for weights up to 2^-6 of the largest, up to 21 units above)
 static __device__ __forceinline__ double weight(float x, double m, double inv_t_log2e, const double *root)
 {
     const double t = fmax(((double)x - m) * inv_t_log2e, -64.0);

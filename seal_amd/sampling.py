@@ -34,7 +34,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     token, in the order of the vocabulary, whose cumulative weight ``exp(logit / temperature)`` passes ``u * total``.  The weights are those of
     the tokens that ``allowed_bits`` (int32 [rows, >= ceil(vocab / 32)], bit v of a row: token v may be drawn) allows, then of the ``top_k`` largest
     (0: all; of equal logits the lower index is the larger), then of the fewest that hold at least ``top_p`` of the weight left (1: all), then of those with at
-    least ``min_p`` of the largest weight (0: all); the largest always stays.  ``temperature`` 0: the first of the largest logits.  Each setting is a number
+    least ``min_p`` of the largest weight (0: all); the largest always stays.  A weight below 2^-45 of the largest is none: its token is not drawn.  ``temperature`` 0: the first of the largest logits.  Each setting is a number
     for all rows or a tensor with one for each row (fp32; ``top_k`` int32).  NaN logits are never drawn, +inf counts as the largest fp32 number.
 
     A row of which no token may be drawn gives token -1 and log-probability -inf.  ``logprobs`` are those of the model: ``logit - logsumexp`` of the whole

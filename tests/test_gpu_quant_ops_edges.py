@@ -201,3 +201,24 @@ def test_weights_are_quantised_alike_on_the_gpu_and_multiply_with_tiny_scales(si
     want = X @ W.T
     got = w4_linear(x.to(DEV), b).double().cpu().numpy()
     assert (np.abs(got - want) <= ops._product_bound(X, W, want, 300, F32)).all()
+
+
+# ---------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("V,rows", [(50, 1), (40000, 1), (40000, 70)])
+def test_weights_below_the_unit_are_not_drawn(V, rows):
+    """weights are multiples of 2^-44 of the largest: exp(-30.8) is one of them, exp(-31.3) is none, so that u = 0 falls on the first token of at least 2^-45; in each of the ways that a
+    row is gone through (a list that one wave finishes, the whole row, rows spread over the card)"""
+    from seal_amd.sampling import sample_tokens
+    x = torch.full((rows, V), -200.0)
+    x[:, V - 1] = 0.0
+    x[:, 3], x[:, 7] = -31.3, -30.8
+    u = torch.zeros(rows, 1)
+    for kw in (dict(), dict(top_k=10), dict(top_k=600), dict(top_p=1 - 2.0 ** -24), dict(min_p=2.0 ** -46)):
+        tok, lp = sample_tokens(x.to(DEV), u.to(DEV), **kw)
+        want = V - 1 if "top_p" in kw else 7               # (the nucleus is the largest alone: it holds 1 - 2^-44 of the weight)
+        assert (tok == want).all(), kw
+        assert torch.allclose(lp.cpu(), x[:, want:want + 1], atol=1e-5)
+    x[:, 7] = -31.3
+    assert (sample_tokens(x.to(DEV), u.to(DEV))[0] == V - 1).all()
