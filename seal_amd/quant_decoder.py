@@ -42,7 +42,7 @@ class QuantStepDecoder(BartStepDecoder):
         if not w.is_cuda:
             raise RuntimeError("QuantStepDecoder: the model must live on the GPU (seal_amd has no CPU path)")
         self.block, self.quantized = block, weights is not None
-        self._states, self._cur = OrderedDict(), None
+        self._states, self._cur, self._side = OrderedDict(), None, None
         self._w4 = {}
         if self.quantized:
             for L in self.layers:
@@ -145,7 +145,9 @@ class QuantStepDecoder(BartStepDecoder):
     def _capture(self, st, dev):
         """warm up, then capture (both write the caches: the caller resets the lengths, and a block starts over with its first token)"""
         with torch.inference_mode(False), torch.no_grad():
-            side = torch.cuda.Stream(device=dev)
+            side = self._side
+            if side is None or side.device != dev:
+                side = self._side = torch.cuda.Stream(device=dev)
             side.wait_stream(torch.cuda.current_stream(dev))
             with torch.cuda.stream(side):
                 for _ in range(2):
@@ -154,7 +156,8 @@ class QuantStepDecoder(BartStepDecoder):
                     self._forward(st)
             torch.cuda.current_stream(dev).wait_stream(side)
             g = torch.cuda.CUDAGraph()
-            with captured(g, capture_error_mode="thread_local"):
+            # (on a stream of the model's device: torch's own capture stream is on the device that was current when it was made, and what runs elsewhere is not captured)
+            with captured(g, stream=side, capture_error_mode="thread_local"):
                 st.logits = self._forward(st)
             st.graph = g
 
