@@ -42,7 +42,7 @@ class QuantStepDecoder(BartStepDecoder):
         if not w.is_cuda:
             raise RuntimeError("QuantStepDecoder: the model must live on the GPU (seal_amd has no CPU path)")
         self.block, self.quantized = block, weights is not None
-        self._states, self._cur, self._side = OrderedDict(), None, None
+        self._states, self._cur, self._side, self._last_stream = OrderedDict(), None, None, None
         self._w4 = {}
         if self.quantized:
             for L in self.layers:
@@ -54,6 +54,16 @@ class QuantStepDecoder(BartStepDecoder):
         if self.quantized:
             return w4_linear(x, self._w4[key], bias, gelu=gelu)
         return F.linear(x, weight, bias)
+
+    def _in_order(self, dev) -> None:
+        """the buffers of a shape go from call to call: one that is made on another stream than the call before waits for what that stream has been given (a caller who
+        captures orders its streams itself)"""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        now = torch.cuda.current_stream(dev)
+        if self._last_stream is not None and self._last_stream != now:
+            now.wait_stream(self._last_stream)
+        self._last_stream = now
 
     # -- one decode's buffers and graph; the narrower continuations of a loop over several decodes are views of them --
     class _State:
@@ -170,6 +180,7 @@ class QuantStepDecoder(BartStepDecoder):
         self.batch, self.beams, self.rows, self.max_len, self.t = B, num_beams, B * num_beams, max_len, 0
         S64, T64 = -(-S // 64) * 64, -(-max_len // 64) * 64
         key = (B, num_beams, S64, T64, enc_hidden.dtype, str(dev))
+        self._in_order(dev)
         self._root = self._cur = None                # (the last decode is over: its shape may go)
         self._make_room(key, dev)
         st = self._states.get(key)
@@ -201,6 +212,7 @@ class QuantStepDecoder(BartStepDecoder):
         st = self._cur
         if self.t >= self.max_len:
             raise RuntimeError(f"QuantStepDecoder: a decode of {self.max_len} positions is over")
+        self._in_order(st.tokens.device)
         st.tokens.copy_(tokens)
         if st.graph is not None:
             st.graph.replay()
@@ -215,6 +227,7 @@ class QuantStepDecoder(BartStepDecoder):
     @torch.no_grad()
     def reorder(self, beam_idx: torch.Tensor) -> None:
         """new row r continues old row beam_idx[r] (HF ``_reorder_cache``): the rows' codes move"""
+        self._in_order(beam_idx.device)
         for own in self._cur.own:
             own.reorder(beam_idx)
 

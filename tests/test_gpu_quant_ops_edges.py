@@ -222,3 +222,45 @@ def test_weights_below_the_unit_are_not_drawn(V, rows):
         assert torch.allclose(lp.cpu(), x[:, want:want + 1], atol=1e-5)
     x[:, 7] = -31.3
     assert (sample_tokens(x.to(DEV), u.to(DEV))[0] == V - 1).all()
+
+
+def test_decodes_of_one_decoder_on_several_streams():
+    """a decode right behind another of the same shape (the same buffers and graph) on another stream, and one that changes streams on its way, without a wait between them: each is what
+    it is alone"""
+    from seal_amd.quant_decoder import QuantStepDecoder
+    model = tiny_bart(130, d_model=128, heads=2, max_positions=160).to(DEV)
+    g = torch.Generator().manual_seed(23)
+    B, S, T = 2, 90, 12
+    work = []
+    for _ in range(4):
+        ids = torch.randint(4, 122, (B, S), generator=g).to(DEV)
+        work.append((ids, torch.ones_like(ids), [torch.randint(4, 122, (2 * B,), generator=g).to(DEV) for _ in range(T)]))
+    order = torch.tensor([1, 0, 3, 3], device=DEV)
+    for graph in (True, False):
+        dec = QuantStepDecoder(model)
+        dec.use_graph = graph
+        enc = [dec.encode(ids, mask) for ids, mask, _ in work]
+
+        def decode(i, streams):
+            ids, mask, toks = work[i]
+            out = []
+            with torch.cuda.stream(streams[0]):
+                dec.start(enc[i], mask, 2, T)
+            for t in range(T):
+                with torch.cuda.stream(streams[t % len(streams)]):
+                    out.append(dec.step(toks[t]).clone())
+                if t == 5:
+                    with torch.cuda.stream(streams[-1]):
+                        dec.reorder(order)
+            return out
+        here = torch.cuda.current_stream()
+        want = [decode(i, [here]) for i in range(4)]
+        torch.cuda.synchronize()
+        a, b, c = (torch.cuda.Stream() for _ in range(3))
+        for _ in range(3):
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(20_000_000)              # (the first decode is still to come when the others are given out)
+            got = [decode(0, [a]), decode(1, [b]), decode(2, [a, b, c]), decode(3, [c])]
+            torch.cuda.synchronize()
+            for x, y in zip(got, want):
+                assert all(torch.equal(p, q) for p, q in zip(x, y))

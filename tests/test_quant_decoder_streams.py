@@ -42,3 +42,26 @@ def test_the_step_is_captured_on_a_stream_of_the_models_device(monkeypatch):
         d._capture(st, torch.device(device))
         assert st.graph is not None and seen[-1] is not None and seen[-1].device == torch.device(device) and entered[-1] is seen[-1]
     assert len(made) == 2                                  # (one stream for a device, not one for every shape)
+
+
+def test_calls_on_another_stream_wait_for_the_one_before(monkeypatch):
+    waits, now, capturing = [], [None], [False]
+
+    class Stream:
+        def __init__(self, name):
+            self.name = name
+
+        def wait_stream(self, other):
+            waits.append((self.name, other.name))
+    a, b = Stream("a"), Stream("b")
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    d = object.__new__(QuantStepDecoder)
+    d._last_stream = None
+    for s in (a, a, b, b, a):
+        now[0] = s
+        d._in_order(torch.device("cuda:0"))
+    assert waits == [("b", "a"), ("a", "b")]
+    now[0], capturing[0] = b, True                         # (a wait for work outside a capture would end it)
+    d._in_order(torch.device("cuda:0"))
+    assert len(waits) == 2
