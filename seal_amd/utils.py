@@ -13,10 +13,8 @@ _CAPTURE = threading.RLock()
 
 @contextlib.contextmanager
 def collector_held():
-    """No collection of cyclic garbage in this process, and no other thread in here, while the block runs: what is dead goes before, what dies meanwhile waits.  The collector
-    is left as it was."""
+    """No collection of cyclic garbage in this process, and no other thread in here, while the block runs: what is dead waits.  The collector is left as it was."""
     with _CAPTURE:
-        gc.collect()
         was = gc.isenabled()
         gc.disable()
         try:
@@ -32,8 +30,8 @@ def captured(graph, **kwargs):
     (``model._seal_step_decoder``), so a decoder that is no longer used, and the graphs that it holds, go when the cyclic collector runs -- after any
     allocation, also one made inside another graph's capture.  The destructor of a ``torch.cuda.CUDAGraph`` synchronises the device on ROCm, which
     a capture forbids; its error leaves a destructor, and that ends the process (seen: "Fatal Python error: Aborted ... Garbage-collecting" under
-    ``tree_hidden_graph``).  So what is dead goes before the capture begins, and the collector waits until it has ended.  Captures of several threads
-    take turns: the first to end would switch the collector on under the others."""
+    ``tree_hidden_graph``).  So the collector waits until the capture has ended (it is not run before: over the half million objects of a searcher that holds a large
+    index that is 50 to 60 ms, for every new shape).  Captures of several threads take turns: the first to end would switch the collector on under the others."""
     with collector_held(), torch.cuda.graph(graph, **kwargs):
         yield
 

@@ -1,5 +1,5 @@
 """Captures of two threads at once (``seal_amd.utils.captured``): the collector is one switch for the process, so the thread that ends first must not switch it on under
-the other's capture, nor collect while the other captures.  On the CPU: the capture itself is replaced by a stand-in."""
+the other's capture.  On the CPU: the capture itself is replaced by a stand-in."""
 import contextlib
 import gc
 import threading
@@ -50,37 +50,13 @@ def test_a_capture_that_ends_leaves_the_collector_off_under_another():
     assert gc.isenabled()
 
 
-def test_no_thread_collects_for_its_own_capture_under_another():
-    calls, inside, go_on = [], threading.Event(), threading.Event()
-    capturing = []
-
-    def collect(*a):
-        calls.append(bool(capturing))
-        return 0
-
-    def first():
-        with utils.captured(object()):
-            capturing.append(1)
-            inside.set()
-            go_on.wait(10)
-            capturing.clear()
-
-    def second():
-        with utils.captured(object()):
-            pass
-    real, gc.collect = gc.collect, collect
-    try:
-        a, b = threading.Thread(target=first), threading.Thread(target=second)
-        a.start()
-        inside.wait(10)
-        b.start()
-        b.join(0.2)
-        go_on.set()
-        a.join(20)
-        b.join(20)
-    finally:
-        gc.collect = real
-    assert not a.is_alive() and not b.is_alive() and calls == [False, False]
+def test_a_capture_does_not_collect(monkeypatch):
+    """neither under another thread's capture nor at all: a full collection is 50 ms and more in a process with many objects, and every new shape would pay it"""
+    calls = []
+    monkeypatch.setattr(gc, "collect", lambda *a: calls.append(a) or 0)
+    with utils.captured(object()):
+        pass
+    assert not calls
 
 
 def test_a_capture_inside_a_held_block_of_the_same_thread():
