@@ -82,7 +82,8 @@ static __device__ __forceinline__ float wave_largest(float m)
 }
 
 // One new token (a decode step): a wave per (slot, head), a lane per dim (two for 128).  The codes of the block before it are only touched where its scale has to grow.
-// Bound by a launch and two round trips to memory (the length, then the scale): 300 slots x 16 heads fp32 7.2 us, 1.8 TB/s.
+// 300 slots x 16 heads fp32: 7.2 us, a launch (3.5 to 4) and what the layout of V costs: a dim's new byte is a write of 32 bytes to memory of its own (10.3 MB written for 0.6 MB of
+// codes, by the counters), behind two round trips (the length, then the scale).
 template <typename T_, int DH>
 __global__ __launch_bounds__(256) void k_kv8_append_one(AppendArgs a)
 {
@@ -330,7 +331,8 @@ __global__ __launch_bounds__(256) void k_kv8_append(AppendArgs a, uint32_t vec)
 // A block's scale is a factor of S's rows (K) or of p (V).
 // Bytes behind `length` or masked may be anything: S is selected, p is 0 there and V's bytes are cleared.
 // Measured: 32 slots x 8 heads of 4001 .. 8192 tokens, dh 128, bf16 80 us, 5.0 TB/s (memory); 1 slot x 16 heads of 32001 tokens bf16 in 32 parts 18.3 us, 3.6 TB/s, the join
-// 3 of them; 40 slots x 16 heads x 15 beams of 500 .. 1024 tokens fp32 20.6 us, 3.3 TB/s (640 workgroups on 256 CUs, and the planes' arithmetic); 20 x 16 heads x 15
+// 3 of them; 40 slots x 16 heads x 15 beams of 500 .. 1024 tokens fp32 20.6 us, 3.3 TB/s (640 workgroups of unequal length on 256 CUs; the vector units issue in a third
+// of the cycles, the matrix units in a tenth); 20 x 16 heads x 15
 // beams of 12 .. 30 tokens 5.0 us, a launch and one tile's round trips.
 // ---------------------------------------------------------------------------------------------------------------------------------
 struct AttendArgs {
@@ -565,7 +567,8 @@ __global__ __launch_bounds__(256, DH == 64 ? 3 : 2) void k_kv8_attend(AttendArgs
 }
 
 // One query on a cache of one tile (a decode step over the short history of each of many rows): the matrix instructions would compute sixteen, and the registers of their
-// operands keep waves away that this case needs -- it is bound by the round trips of its loads, 300 rows x 16 heads being one wave each: 7.8 us.  Plain
+// operands keep waves away that this case needs -- 300 rows x 16 heads of 1 .. 17 tokens are one wave each: 7.8 us, a launch and 26 MB read (by the counters),
+// three times what the tokens hold: the first sixteen tokens of V lie in every 16 bytes of its tile, so all 4 KB of it are read.  Plain
 // multiply-adds on the same loads: lane (g, c) has dims 16 g .. of token c of each sixteen, then tokens 4 g .. of dim c.
 template <typename T_, int DH>
 __global__ __launch_bounds__(256) void k_kv8_attend_one(AttendArgs a)

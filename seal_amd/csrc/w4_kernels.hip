@@ -103,7 +103,8 @@ static __device__ __forceinline__ void put(float v, const T *bias, uint32_t gelu
 }
 
 // More than 1024 columns: a workgroup of W waves has NT tiles of 16 outputs and 16 rows of x, the waves take the 128-column chunks in turn and their sums meet
-// in LDS.  GS: matrix instructions per scale group (group / 32).  Rows of x beyond the last repeat it: what a matrix instruction makes of them is not stored.
+// in LDS.  GS: matrix instructions per scale group (group / 32).  Rows of x beyond the last repeat it: what a matrix instruction makes of them is not stored.  1 x 1024 x 4096
+// fp32 6.3 us, 64 workgroups each of whose waves has two chunks: latency; 300 x 1024 x 4096 32 (the library's fp32 product 34).
 template <typename T, int NT, int GS, int W>
 __global__ __launch_bounds__(64 * W) void k_w4_linear_long(const T *x, uint64_t x_stride, const uint32_t *codes, const uint16_t *scales, const T *bias,
                                                            uint32_t M, uint32_t N, uint32_t K, uint32_t vec, uint32_t gelu, T *y)
@@ -164,7 +165,9 @@ __global__ __launch_bounds__(64 * W) void k_w4_linear_long(const T *x, uint64_t 
 // At most 1024 columns: `kw` of a workgroup's eight waves (1, 2, 4 or 8) have one 128-column chunk each, 8 / kw such teams NT tiles of 16 outputs x MT tiles of 16 rows of
 // x.  A wave's chunk of x stays in its registers as planes (splitting fp32 into them costs more instructions than the products) while the workgroup goes
 // from tiles to tiles, every gridDim.x * 8 / kw * NT; the next round's codes are on their way while it works on these.  The waves' sums of two rounds lie side by side in LDS:
-// one barrier a round.  1 x 50265 x 1024 fp32 in 10.6 us, 2.6 TB/s of codes and scales; a launch and the first loads are 4 of them.
+// one barrier a round.  1 x 50265 x 1024 fp32 in 10.6 us, 2.6 TB/s of codes and scales; a launch and the first loads are 4 of them, its 1571 pairs of tiles
+// are 3.07 rounds of 512 workgroups (the last of 35 alone), and the joining sums all 16 columns though one is stored.  Vector units issue in a quarter of the cycles.
+// From 17 rows on fp32 decodes the codes again for every 16 rows: 64 x 50265 x 1024 33 us, 300 x 50265 x 1024 143.
 template <typename T, int NT, int MT, int GS>
 __global__ __launch_bounds__(512, 2) void k_w4_linear_many(const T *x, uint64_t x_stride, const uint32_t *codes, const uint16_t *scales, const T *bias,
                                                            uint32_t M, uint32_t N, uint32_t K, uint32_t kw, uint32_t vec, uint32_t gelu, T *y)

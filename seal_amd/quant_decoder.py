@@ -2,7 +2,10 @@
 
 ``BartStepDecoder``'s fused step holds at most 17 decoder positions and 64 encoder tokens and reads its weights at 16 or 32 bits.  ``QuantStepDecoder`` keeps the
 self-attention history and the encoder's keys and values in ``KV8Cache`` (any length, a quarter of the bytes of fp32) and, with ``weights="w4"``, runs every product
-of a step through ``w4_linear`` (an eighth of the bytes): for long inputs, long outputs and few rows, where a step is bound by reading them.  Both
+of a step through ``w4_linear`` (an eighth of the bytes): for long inputs, long outputs and few rows, where a step is bound by reading them.
+BART-large, us a step, fp32 step / this one: 1 row 1324 / 639, 60 rows 1318 / 955, inputs of 1000 tokens 1828 / 689 (1 row) and 4945 / 2066 (300 rows), 200 positions
+5508 / 2241 (300 rows) -- but 300 rows of 30 tokens and 16 positions 1570 / 1935, and 1575 / 2496 where a beam search reorders the rows (``reorder`` copies whole caches): such decodes
+are the fp32 step's.  Both
 round: the scores are those of a model whose weights have 4 and whose keys and values have 8 bits.  The encoder, the projection of its states and the rescoring
 forward (``keys.py``) stay what ``BartStepDecoder`` runs.
 

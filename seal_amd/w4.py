@@ -63,8 +63,8 @@ def quantize_w4(weight: torch.Tensor, group: int = 32) -> W4Weight:
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None, gelu: bool = False) -> torch.Tensor:
-    """``F.linear(x, weight, bias)`` (and its erf GELU) for ``x`` fp32 or bf16 [rows, in_features], rows may be strided; ``bias`` of x's type.  Made for 1 .. 64 rows; up
-    to 2^19 work.  Returns a new [rows, out_features] of x's type.  A row of x that is not finite gives
+    """``F.linear(x, weight, bias)`` (and its erf GELU) for ``x`` fp32 or bf16 [rows, in_features], rows may be strided; ``bias`` of x's type.  Made for 1 .. 64 rows (a wide
+    bf16 layer, 50265 x 1024, takes 35 us at 60 rows, the library's 16-bit product 20); up to 2^19 work.  Returns a new [rows, out_features] of x's type.  A row of x that is not finite gives
     a row that is not (fp32: NaN; bf16: what inf * w sums to).  No gradient: an input that requires one is refused unless it is called under ``torch.no_grad()``."""
     codes, dt = weight.codes, x.dtype
     if x.dim() != 2 or x.shape[1] != weight.in_features or (dt != torch.float32 and dt != torch.bfloat16) or x.device != codes.device:
